@@ -20,7 +20,8 @@ __all__ = [
     "selftest_bounded_wait", "mxfp4_bf16_gemm", "mxfp4_sf_storage_bytes", "mxfp4_quantize",
     "quantize_tensor_mxfp4", "mxf8f4_bf16_gemm", "mxfp8_quantize", "quantize_tensor_mxfp8",
     "nvfp4_bf16_gemm_gather", "peer_barrier", "ipc_get_handle", "ipc_open", "ipc_close",
-    "selftest_skinny_partial_wait",
+    "selftest_skinny_partial_wait", "NORM_KINDS", "NORM_OUTPUTS", "block_norm",
+    "block_norm_backward", "block_norm_backward_workspace_bytes",
 ]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -103,6 +104,12 @@ def load():
     L.blackhole_sm100_ipc_open.argtypes = [vp, i64, ctypes.POINTER(ctypes.c_void_p)]
     L.blackhole_sm100_ipc_close.restype = i32
     L.blackhole_sm100_ipc_close.argtypes = [vp]
+    L.blackhole_sm100_block_norm.restype = i32
+    L.blackhole_sm100_block_norm.argtypes = [vp, vp]
+    L.blackhole_sm100_block_norm_backward.restype = i32
+    L.blackhole_sm100_block_norm_backward.argtypes = [vp, vp]
+    L.blackhole_sm100_block_norm_backward_workspace_bytes.restype = i64
+    L.blackhole_sm100_block_norm_backward_workspace_bytes.argtypes = [i32, i32, i32, i32]
     L.blackhole_sm100_abi_version.restype = i32
     L.blackhole_sm100_abi_version.argtypes = []
     _lib = L
@@ -399,3 +406,7 @@ def quantize_tensor(X, stream=None):
     scales = torch.empty(2, dtype=torch.float32, device=X.device)
     nvfp4_quantize(X, rows, K, packed, sf, scales, x_is_bf16=(X.dtype == torch.bfloat16), stream=stream)
     return packed, sf, scales
+
+
+from .fused import (NORM_KINDS, NORM_OUTPUTS, block_norm, block_norm_backward,  # noqa: E402
+                    block_norm_backward_workspace_bytes)

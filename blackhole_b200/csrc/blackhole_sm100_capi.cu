@@ -8,6 +8,7 @@
 #include <blackhole/sm100/nvfp4_quant.hpp>
 #include <blackhole/sm100/bounded_wait_selftest.hpp>
 #include <blackhole/sm100/peer_barrier.hpp>
+#include <blackhole/sm100/block_norm.hpp>
 
 #include <cstring>
 #include <map>
@@ -296,6 +297,22 @@ int blackhole_sm100_selftest_skinny_partial_wait(int M, int N, int K, const void
 int blackhole_sm100_selftest_bounded_wait(uint64_t limit_ns, uint64_t* result,
                                           cudaStream_t stream) {
   return static_cast<int>(blackhole::sm100::bounded_wait_selftest(limit_ns, result, stream));
+}
+
+int blackhole_sm100_block_norm(const blackhole_sm100_block_norm_args* args, cudaStream_t stream) {
+  if (!args) return static_cast<int>(cudaErrorInvalidValue);
+  return static_cast<int>(blackhole::sm100::block_norm(*args, stream));
+}
+
+int blackhole_sm100_block_norm_backward(const blackhole_sm100_block_norm_backward_args* args,
+                                        cudaStream_t stream) {
+  if (!args) return static_cast<int>(cudaErrorInvalidValue);
+  return static_cast<int>(blackhole::sm100::block_norm_backward(*args, stream));
+}
+
+int64_t blackhole_sm100_block_norm_backward_workspace_bytes(int rows, int H, int has_gate,
+                                                            int gate_rows) {
+  return blackhole::sm100::block_norm_backward_workspace_bytes(rows, H, has_gate, gate_rows);
 }
 
 int blackhole_sm100_abi_version(void) { return BLACKHOLE_SM100_ABI_VERSION; }

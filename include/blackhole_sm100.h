@@ -221,6 +221,65 @@ BLACKHOLE_SM100_API int blackhole_sm100_mxfp4_quantize(const void* X, int x_is_b
                                                        int K, void* packed, void* sf,
                                                        cudaStream_t stream);
 
+/* Norms before and after a block, fused with its gate and residual scale (no counterpart in the
+ * reference): per row of H features
+ *     p = o, or norm(o) * post_weight + post_bias with post_norm
+ *     h = x + scale * gate * p
+ *     out = norm(h) * weight + bias
+ * norm(v) is v / sqrt(mean(v^2) + eps) (kind 0, RMS) or (v - mean) / sqrt(var + eps) (kind 1).
+ *   x      : rows x H residual stream, BF16 (x_is_bf16) or FP32; h has its type, may be x itself
+ *   o      : rows x H BF16, the block's result; NULL: h = x, and gate, h, post_* must be NULL
+ *   gate   : NULL (1), or rows of H features (BF16 if gate_is_bf16, else FP32): row r of x takes
+ *            gate row r / gate_rows; gate_rows = 0: one gate row for all, 1: one per row
+ *   weight, bias, post_weight, post_bias : H values (BF16 if param_is_bf16, else FP32), NULL: 1 / 0
+ *   out    : NULL, or the result in out_format: 0 BF16, 1 FP32, or the A operand of the next
+ *            product: 2 NVFP4 (with global_scale, which belongs into that product's alpha),
+ *            3 MXFP4, 4 MXFP8, quantised from the FP32 result as by the quantisers below, with
+ *            its scale factors in sf (sf_storage_bytes / mxfp4_sf_storage_bytes of (rows, H);
+ *            padding written 0); sf is NULL for formats 0 and 1
+ *   stats  : NULL, or rows x 4 FP32: mean and 1 / sqrt(var + eps) of the post norm, then of the
+ *            norm (0, and 0 for a post norm that is not there; the mean of an RMS norm is 0)
+ * rows >= 1; H % 8 == 0 (NVFP4 % 16, MX % 32), 8 <= H <= 16384; contiguous, 16-byte aligned,
+ * outputs not over inputs (h == x excepted).  Statistics and sums are FP32.  Errors:
+ * cudaErrorInvalidValue for what breaks these rules, else the launch status.  Asynchronous and
+ * stream-ordered, a programmatic dependent of the kernel before it like the products. */
+typedef struct blackhole_sm100_block_norm_args {
+  int rows, H, kind, x_is_bf16, param_is_bf16, gate_is_bf16, post_norm, gate_rows, out_format;
+  float eps, scale, global_scale;
+  const void *x, *o, *gate, *weight, *bias, *post_weight, *post_bias;
+  void *h, *out, *sf;
+  float* stats;
+} blackhole_sm100_block_norm_args;
+BLACKHOLE_SM100_API int blackhole_sm100_block_norm(const blackhole_sm100_block_norm_args* args,
+                                                   cudaStream_t stream);
+
+/* Its backward pass.  h (the stored stream; x where o was NULL) and stats as block_norm left them,
+ * o, gate, weight, post_weight, post_bias, scale, kind, post_norm, gate_rows as given to it.
+ *   dy, dh : gradients of out (BF16) and of h (type of x); either may be NULL (zero)
+ *   dx     : gradient of x (type of x; may be dh itself);  d_o : gradient of o, BF16
+ *   dweight, dbias, dpost_weight, dpost_bias : NULL, or H FP32 values (overwritten)
+ *   dgate  : NULL, or FP32 of the gate's shape (overwritten)
+ *   workspace : device memory of blackhole_sm100_block_norm_backward_workspace_bytes(...) bytes,
+ *            16-byte aligned, for the column sums (NULL where none of those gradients, or only a
+ *            dgate with gate_rows = 1, is asked for); contents do not matter.  Calls sharing one
+ *            must be ordered, replays of captured graphs among them.
+ * Sums over rows are FP32, in an order fixed by the sizes: results are reproducible. */
+typedef struct blackhole_sm100_block_norm_backward_args {
+  int rows, H, kind, x_is_bf16, param_is_bf16, gate_is_bf16, post_norm, gate_rows;
+  float scale;
+  const void *h, *dy, *dh, *o, *gate, *weight, *post_weight, *post_bias;
+  const float* stats;
+  void *dx, *d_o;
+  float *dweight, *dbias, *dpost_weight, *dpost_bias, *dgate;
+  void* workspace;
+  int64_t workspace_bytes;
+} blackhole_sm100_block_norm_backward_args;
+BLACKHOLE_SM100_API int blackhole_sm100_block_norm_backward(
+    const blackhole_sm100_block_norm_backward_args* args, cudaStream_t stream);
+BLACKHOLE_SM100_API int64_t blackhole_sm100_block_norm_backward_workspace_bytes(int rows, int H,
+                                                                                int has_gate,
+                                                                                int gate_rows);
+
 /* ABI version of the loaded library (BLACKHOLE_SM100_ABI_VERSION). */
 BLACKHOLE_SM100_API int blackhole_sm100_abi_version(void);
 
