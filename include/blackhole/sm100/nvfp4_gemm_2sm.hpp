@@ -103,13 +103,17 @@ struct Nvfp4Gemm2SmTraitsT {
   // epilogue staging: one 32-row x 64-column BF16 box (4 KB, 128B-swizzled) per epilogue warp
   static constexpr int StoreBoxBytes = 32 * 64 * 2;
   static constexpr int StagingBytes = NumEpiWarps * StoreBoxBytes;
+  // The boxes start on a multiple of 1024 bytes: the 128B swizzle pattern follows the
+  // shared-memory address, so on an odd multiple of 512 every 64-byte half of a row would land
+  // in the other's place (MXFP8 x MXFP4's scale factors take 1.5 KB per stage).
+  static constexpr int StagingOffset = (Stages * StageBytes + 1023) / 1024 * 1024;
 
   // stage full/empty, accumulator full/empty, drain, TMEM slot + abort flag, then (copy warp)
   // scale-factor buffer full/empty, the copy warp's drain barrier and the stages' scale-factor
   // full barriers
   static constexpr int BarrierBytes =
       8 * (2 * Stages + 4) + 16 + 8 * (2 * SfBufs + 1) + (SfCopyWarp ? 8 * Stages : 0);
-  static constexpr int SmemBytes = Stages * StageBytes + StagingBytes + BarrierBytes + 1024;
+  static constexpr int SmemBytes = StagingOffset + StagingBytes + BarrierBytes + 1024;
 
   static_assert(SmemBytes <= arch_traits<Arch::kSm100>::max_smem_per_cta, "smem budget");
   static_assert(SfCol + SfBufs * SfStride <= TmemCols, "TMEM budget");
@@ -191,7 +195,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
   const uint32_t sB = sA + S * KT::ABytes;
   const uint32_t sSFA = sB + S * KT::BBytes;
   const uint32_t sSFB = sSFA + S * KT::SFABytes;
-  const uint32_t sStage = sSFB + S * KT::SFBBytes;   // epilogue staging boxes
+  const uint32_t sStage = base + KT::StagingOffset;   // epilogue staging boxes
   const uint32_t bars = sStage + KT::StagingBytes;
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
@@ -496,10 +500,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
       if (!wait_bounded_warp(acc_full, acc_phase, abort_flag, p.status, kStatusEpilogueTimeout)) break;
       tc_fence_after();
       uint32_t v0[32], v1[32], v2[32], v3[32];
-      // Measured on B200: the two-SM kind::mxf8f6f4 MMA (N = 256) leaves output column n in
-      // accumulator column n XOR 32 (32-column groups swapped pairwise inside each half; lanes
-      // and halves as for kind::mxf4nvf4), so that kind reads the groups crosswise.
-      constexpr uint32_t x = KT::Fmt::Kind == MmaKind::kMxf8f6f4 ? 32u : 0u;
       const uint32_t acc_col = KT::OverlapAcc ? (acc_phase ? KT::AccStageStride : 0u) : KT::AccCol;
       const uint32_t t_row = tmem + (static_cast<uint32_t>(32 * q) << 16) + acc_col + 128 * half;
       if constexpr (KT::OverlapAcc) {
@@ -515,11 +515,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
           if (lane == 0) mbar_arrive_cluster(leader_acc_empty);
         }
         if (shared_hi) {
-          tmem_ld_32x32b_x32(t_row + (64 ^ x), v2);
-          tmem_ld_32x32b_x32(t_row + (96 ^ x), v3);
+          tmem_ld_32x32b_x32(t_row + 64, v2);
+          tmem_ld_32x32b_x32(t_row + 96, v3);
         } else {
-          tmem_ld_32x32b_x32(t_row + (0 ^ x), v0);
-          tmem_ld_32x32b_x32(t_row + (32 ^ x), v1);
+          tmem_ld_32x32b_x32(t_row + 0, v0);
+          tmem_ld_32x32b_x32(t_row + 32, v1);
         }
         tmem_ld_wait();
         if (holds) {
@@ -528,11 +528,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
           if (lane == 0) mbar_arrive_cluster(leader_acc_empty);
         }
         if (shared_hi) {
-          tmem_ld_32x32b_x32(t_row + (0 ^ x), v0);
-          tmem_ld_32x32b_x32(t_row + (32 ^ x), v1);
+          tmem_ld_32x32b_x32(t_row + 0, v0);
+          tmem_ld_32x32b_x32(t_row + 32, v1);
         } else {
-          tmem_ld_32x32b_x32(t_row + (64 ^ x), v2);
-          tmem_ld_32x32b_x32(t_row + (96 ^ x), v3);
+          tmem_ld_32x32b_x32(t_row + 64, v2);
+          tmem_ld_32x32b_x32(t_row + 96, v3);
         }
         tmem_ld_wait();
         reg_fence(v0);
@@ -540,10 +540,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
         reg_fence(v2);
         reg_fence(v3);
       } else {
-        tmem_ld_32x32b_x32(t_row + (0 ^ x), v0);
-        tmem_ld_32x32b_x32(t_row + (32 ^ x), v1);
-        tmem_ld_32x32b_x32(t_row + (64 ^ x), v2);
-        tmem_ld_32x32b_x32(t_row + (96 ^ x), v3);
+        tmem_ld_32x32b_x32(t_row + 0, v0);
+        tmem_ld_32x32b_x32(t_row + 32, v1);
+        tmem_ld_32x32b_x32(t_row + 64, v2);
+        tmem_ld_32x32b_x32(t_row + 96, v3);
         tmem_ld_wait();
         reg_fence(v0);
         reg_fence(v1);
