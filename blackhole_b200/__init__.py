@@ -21,7 +21,9 @@ __all__ = [
     "quantize_tensor_mxfp4", "mxf8f4_bf16_gemm", "mxfp8_quantize", "quantize_tensor_mxfp8",
     "nvfp4_bf16_gemm_gather", "peer_barrier", "ipc_get_handle", "ipc_open", "ipc_close",
     "selftest_skinny_partial_wait", "NORM_KINDS", "NORM_OUTPUTS", "block_norm",
-    "block_norm_backward", "block_norm_backward_workspace_bytes",
+    "block_norm_backward", "block_norm_backward_workspace_bytes", "ACTIVATIONS",
+    "nvfp4_bf16_gemm_fused", "mxfp4_bf16_gemm_fused", "mxf8f4_bf16_gemm_fused",
+    "gemm_fused_backward", "gemm_fused_backward_workspace_bytes",
 ]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -104,6 +106,14 @@ def load():
     L.blackhole_sm100_ipc_open.argtypes = [vp, i64, ctypes.POINTER(ctypes.c_void_p)]
     L.blackhole_sm100_ipc_close.restype = i32
     L.blackhole_sm100_ipc_close.argtypes = [vp]
+    for fmt in ("nvfp4", "mxfp4", "mxf8f4"):
+        f = getattr(L, f"blackhole_sm100_{fmt}_bf16_gemm_fused")
+        f.restype = i32
+        f.argtypes = [i32, i32, i32, vp, vp, vp, vp, vp, ctypes.c_float, vp, i32, vp, i64, vp]
+    L.blackhole_sm100_gemm_fused_backward.restype = i32
+    L.blackhole_sm100_gemm_fused_backward.argtypes = [i32, i32, vp, vp, vp, vp, i32, i32, vp, i64, vp]
+    L.blackhole_sm100_gemm_fused_backward_workspace_bytes.restype = i64
+    L.blackhole_sm100_gemm_fused_backward_workspace_bytes.argtypes = [i32, i32]
     L.blackhole_sm100_block_norm.restype = i32
     L.blackhole_sm100_block_norm.argtypes = [vp, vp]
     L.blackhole_sm100_block_norm_backward.restype = i32
@@ -408,5 +418,7 @@ def quantize_tensor(X, stream=None):
     return packed, sf, scales
 
 
-from .fused import (NORM_KINDS, NORM_OUTPUTS, block_norm, block_norm_backward,  # noqa: E402
-                    block_norm_backward_workspace_bytes)
+from .fused import (ACTIVATIONS, NORM_KINDS, NORM_OUTPUTS, block_norm,  # noqa: E402
+                    block_norm_backward, block_norm_backward_workspace_bytes, gemm_fused_backward,
+                    gemm_fused_backward_workspace_bytes, mxf8f4_bf16_gemm_fused,
+                    mxfp4_bf16_gemm_fused, nvfp4_bf16_gemm_fused)

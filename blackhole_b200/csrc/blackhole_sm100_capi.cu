@@ -299,6 +299,53 @@ int blackhole_sm100_selftest_bounded_wait(uint64_t limit_ns, uint64_t* result,
   return static_cast<int>(blackhole::sm100::bounded_wait_selftest(limit_ns, result, stream));
 }
 
+int blackhole_sm100_nvfp4_bf16_gemm_fused(int M, int N, int K, const void* A, const void* SFA,
+                                        const void* B, const void* SFB, void* D, float alpha,
+                                        const blackhole_sm100_epilogue* epilogue, int schedule,
+                                        void* workspace, int64_t workspace_bytes,
+                                        cudaStream_t stream) {
+  if (schedule < 0 || schedule > 4) return static_cast<int>(cudaErrorInvalidValue);
+  return static_cast<int>(
+      blackhole::sm100::block_scaled_bf16_gemm_fused<blackhole::sm100::Nvfp4Format>(
+          M, N, K, A, SFA, B, SFB, D, alpha, epilogue,
+          static_cast<blackhole::sm100::Nvfp4Schedule>(schedule), workspace, workspace_bytes, stream));
+}
+
+int blackhole_sm100_mxfp4_bf16_gemm_fused(int M, int N, int K, const void* A, const void* SFA,
+                                        const void* B, const void* SFB, void* D, float alpha,
+                                        const blackhole_sm100_epilogue* epilogue, int schedule,
+                                        void* workspace, int64_t workspace_bytes,
+                                        cudaStream_t stream) {
+  if (schedule < 0 || schedule > 4) return static_cast<int>(cudaErrorInvalidValue);
+  return static_cast<int>(
+      blackhole::sm100::block_scaled_bf16_gemm_fused<blackhole::sm100::Mxfp4Format>(
+          M, N, K, A, SFA, B, SFB, D, alpha, epilogue,
+          static_cast<blackhole::sm100::Nvfp4Schedule>(schedule), workspace, workspace_bytes, stream));
+}
+
+int blackhole_sm100_mxf8f4_bf16_gemm_fused(int M, int N, int K, const void* A, const void* SFA,
+                                        const void* B, const void* SFB, void* D, float alpha,
+                                        const blackhole_sm100_epilogue* epilogue, int schedule,
+                                        void* workspace, int64_t workspace_bytes,
+                                        cudaStream_t stream) {
+  if (schedule < 0 || schedule > 4) return static_cast<int>(cudaErrorInvalidValue);
+  return static_cast<int>(
+      blackhole::sm100::block_scaled_bf16_gemm_fused<blackhole::sm100::Mxf8f4Format>(
+          M, N, K, A, SFA, B, SFB, D, alpha, epilogue,
+          static_cast<blackhole::sm100::Nvfp4Schedule>(schedule), workspace, workspace_bytes, stream));
+}
+
+int blackhole_sm100_gemm_fused_backward(int M, int N, const void* dD, const void* Z, void* dZ,
+                                        float* dbias, int activation, int gated, void* workspace,
+                                        int64_t workspace_bytes, cudaStream_t stream) {
+  return static_cast<int>(blackhole::sm100::gemm_fused_backward(
+      M, N, dD, Z, dZ, dbias, activation, gated, workspace, workspace_bytes, stream));
+}
+
+int64_t blackhole_sm100_gemm_fused_backward_workspace_bytes(int M, int N) {
+  return blackhole::sm100::gemm_fused_backward_workspace_bytes(M, N);
+}
+
 int blackhole_sm100_block_norm(const blackhole_sm100_block_norm_args* args, cudaStream_t stream) {
   if (!args) return static_cast<int>(cudaErrorInvalidValue);
   return static_cast<int>(blackhole::sm100::block_norm(*args, stream));

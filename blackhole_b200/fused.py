@@ -1,6 +1,7 @@
-"""What stands between two block-scaled products of a transformer: the norms before and after a
-block with its gate and residual scale, forward and backward, over the C ABI of
-include/blackhole_sm100.h.
+"""What stands between the accumulators of one block-scaled product of a transformer and the
+operand of the next: the products with bias, activation and residual in their epilogue, the
+gradient through that epilogue, and the norms before and after a block with its gate and residual
+scale, forward and backward, over the C ABI of include/blackhole_sm100.h.
 
 Buffers are torch tensors (checked: CUDA tensors of the current device, contiguous, of the
 documented type and at least the documented size) or raw integer device pointers (taken as they
@@ -10,15 +11,23 @@ from __future__ import annotations
 
 import ctypes
 
-from . import BlackholeError, _stream, load
+from . import SCHEDULES, BlackholeError, _ptr, _stream, load
 
-__all__ = ["NORM_KINDS", "NORM_OUTPUTS", "block_norm", "block_norm_backward",
+__all__ = ["ACTIVATIONS", "nvfp4_bf16_gemm_fused", "mxfp4_bf16_gemm_fused", "mxf8f4_bf16_gemm_fused",
+           "gemm_fused_backward", "gemm_fused_backward_workspace_bytes", "NORM_KINDS", "NORM_OUTPUTS", "block_norm", "block_norm_backward",
            "block_norm_backward_workspace_bytes"]
 
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 NORM_KINDS = {"rms": 0, "layer": 1}
 NORM_OUTPUTS = {"bf16": 0, "f32": 1, "nvfp4": 2, "mxfp4": 3, "mxfp8": 4}
 
 _vp, _i32, _f32, _i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
+
+
+class Epilogue(ctypes.Structure):
+    """blackhole_sm100_epilogue"""
+    _fields_ = [(n, _i32) for n in ("activation", "gated", "bias_is_bf16")] + [("beta", _f32)] + \
+               [(n, _vp) for n in ("bias", "residual", "Z")]
 
 
 class BlockNormArgs(ctypes.Structure):
@@ -91,6 +100,100 @@ def _gate_elements(rows, H, gate_rows):
 
 def _blocked_bytes(rows, H, vec):
     return -(-rows // 128) * -(-(H // vec) // 4) * 512
+
+
+def _gemm_fused(name, M, N, K, A, SFA, B, SFB, D, alpha, bias, activation, gated, residual, beta, Z,
+                bias_is_bf16, schedule, workspace, workspace_bytes, stream):
+    M, N = int(M), int(N)
+    b = _Buffers(stream)
+    bf16 = b.torch.bfloat16
+    n_out = N // 2 if gated else N
+    p_d, p_res, p_z = b("D", D, M * n_out, bf16), b("residual", residual, M * n_out, bf16), b("Z", Z, M * N, bf16)
+    p_bias = b("bias", bias, N, kind="bias")
+    if workspace is not None and hasattr(workspace, "numel") and not workspace_bytes:
+        workspace_bytes = workspace.numel() * workspace.element_size()
+    epi = Epilogue(ACTIVATIONS[activation], int(bool(gated)), b.is_bf16("bias", bias_is_bf16), beta,
+                   p_bias, p_res, p_z)
+    rc = getattr(load(), name)(M, N, int(K), _ptr(A), _ptr(SFA), _ptr(B), _ptr(SFB), p_d, alpha,
+                               ctypes.byref(epi), SCHEDULES[schedule],
+                               _ptr(workspace) if workspace is not None else None,
+                               int(workspace_bytes), _stream(stream))
+    if rc != 0:
+        raise BlackholeError(name, rc)
+
+
+def nvfp4_bf16_gemm_fused(M: int, N: int, K: int, A, SFA, B, SFB, D, alpha: float = 1.0, bias=None,
+                          activation: str = "none", gated: bool = False, residual=None,
+                          beta: float = 1.0, Z=None, bias_is_bf16: bool = False,
+                          schedule: str = "auto", workspace=None, workspace_bytes: int = 0,
+                          stream=None) -> None:
+    """nvfp4_bf16_gemm_ex with an epilogue fused into it:
+
+        z = alpha * A . B^T + bias
+        u = act(z), or gated: u[:, j] = act(z[:, 2j]) * z[:, 2j + 1]   (N / 2 columns)
+        D = bf16(u + beta * residual)
+
+    activation: "none", "relu", "gelu" (erf), "gelu_tanh", "silu".  gated: gate row j of the
+    weights is row 2j of B, up row j row 2j + 1 (N % 16 == 0).  bias: N values, BF16 or FP32
+    (bias_is_bf16 only matters for a raw pointer); residual: BF16 of D's shape, may be D itself;
+    Z: BF16 M x N, receives z for gemm_fused_backward."""
+    _gemm_fused("blackhole_sm100_nvfp4_bf16_gemm_fused", M, N, K, A, SFA, B, SFB, D, alpha, bias,
+                activation, gated, residual, beta, Z, bias_is_bf16, schedule, workspace,
+                workspace_bytes, stream)
+
+
+def mxfp4_bf16_gemm_fused(M: int, N: int, K: int, A, SFA, B, SFB, D, alpha: float = 1.0, bias=None,
+                          activation: str = "none", gated: bool = False, residual=None,
+                          beta: float = 1.0, Z=None, bias_is_bf16: bool = False,
+                          schedule: str = "auto", workspace=None, workspace_bytes: int = 0,
+                          stream=None) -> None:
+    """mxfp4_bf16_gemm with the epilogue of nvfp4_bf16_gemm_fused."""
+    _gemm_fused("blackhole_sm100_mxfp4_bf16_gemm_fused", M, N, K, A, SFA, B, SFB, D, alpha, bias,
+                activation, gated, residual, beta, Z, bias_is_bf16, schedule, workspace,
+                workspace_bytes, stream)
+
+
+def mxf8f4_bf16_gemm_fused(M: int, N: int, K: int, A, SFA, B, SFB, D, alpha: float = 1.0, bias=None,
+                           activation: str = "none", gated: bool = False, residual=None,
+                           beta: float = 1.0, Z=None, bias_is_bf16: bool = False,
+                           schedule: str = "auto", workspace=None, workspace_bytes: int = 0,
+                           stream=None) -> None:
+    """mxf8f4_bf16_gemm with the epilogue of nvfp4_bf16_gemm_fused."""
+    _gemm_fused("blackhole_sm100_mxf8f4_bf16_gemm_fused", M, N, K, A, SFA, B, SFB, D, alpha, bias,
+                activation, gated, residual, beta, Z, bias_is_bf16, schedule, workspace,
+                workspace_bytes, stream)
+
+
+def gemm_fused_backward_workspace_bytes(M: int, N: int) -> int:
+    """Workspace bytes of gemm_fused_backward's dbias (0 when none); negative for sizes it refuses."""
+    return int(load().blackhole_sm100_gemm_fused_backward_workspace_bytes(int(M), int(N)))
+
+
+def gemm_fused_backward(M: int, N: int, dD, Z, dZ, dbias=None, activation: str = "none",
+                        gated: bool = False, workspace=None, workspace_bytes: int = 0,
+                        stream=None) -> None:
+    """Gradient through a fused product's epilogue, from the Z it kept: dZ = dD * act'(Z) (gated:
+    of the pairs), BF16 M x N, and dbias (N FP32, overwritten; None: not wanted) its column sums.
+    dD: BF16 of D's shape.  dZ may be Z, or dD when not gated.  workspace:
+    gemm_fused_backward_workspace_bytes bytes, or None: allocated for this call from torch's
+    caching allocator on the current stream."""
+    M, N = int(M), int(N)
+    b = _Buffers(stream)
+    bf16 = b.torch.bfloat16
+    p_d, p_z, p_dz = b("dD", dD, M * (N // 2 if gated else N), bf16), b("Z", Z, M * N, bf16), b("dZ", dZ, M * N, bf16)
+    p_db = b("dbias", dbias, N, b.torch.float32)
+    if workspace is None and p_db:
+        need = gemm_fused_backward_workspace_bytes(M, N)
+        if need > 0:
+            workspace = _workspace(b, need, stream)
+    if workspace is not None and type(workspace) is not int:
+        workspace_bytes = workspace.numel() * workspace.element_size()
+        workspace = b("workspace", workspace, 0, workspace.dtype)
+    rc = load().blackhole_sm100_gemm_fused_backward(M, N, p_d, p_z, p_dz, p_db, ACTIVATIONS[activation],
+                                                    int(bool(gated)), workspace, int(workspace_bytes),
+                                                    _stream(stream))
+    if rc != 0:
+        raise BlackholeError("blackhole_sm100_gemm_fused_backward", rc)
 
 
 def block_norm(rows: int, H: int, x, out=None, weight=None, bias=None, kind: str = "rms",

@@ -34,6 +34,7 @@
 
 #include <blackhole/common/sf_layout.hpp>
 #include <blackhole/sm100/column_sum.hpp>
+#include <blackhole/sm100/gemm_epilogue.hpp>
 #include <blackhole/sm100/nvfp4_gemm_common.hpp>
 #include <blackhole/sm100/nvfp4_quant.hpp>
 #include <blackhole_sm100.h>
@@ -44,14 +45,6 @@ constexpr int kNormMaxH = 16384;
 constexpr int kNormSliceH = 8192;     // columns one CTA works on: 512 threads x 16
 
 enum NormOut : int { kOutBf16 = 0, kOutF32 = 1, kOutNvfp4 = 2, kOutMxfp4 = 3, kOutMxfp8 = 4 };
-
-// Bytes of an element range do not meet (an output may not be written over an input that other
-// rows still read).
-inline bool ranges_overlap(const void* a, int64_t an, const void* b, int64_t bn) {
-  if (!a || !b || an <= 0 || bn <= 0) return false;
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + static_cast<uintptr_t>(bn) && y < x + static_cast<uintptr_t>(an);
-}
 
 namespace norm_detail {
 
@@ -118,9 +111,9 @@ inline cudaError_t block_norm_check(const blackhole_sm100_block_norm_args& a) {
   const int64_t xb = n * (a.x_is_bf16 ? 2 : 4);
   const int64_t yb = a.out_format == kOutBf16 ? n * 2 : a.out_format == kOutF32 ? n * 4
                      : a.out_format == kOutMxfp8 ? n : n / 2;
-  if (a.h && a.h != a.x && ranges_overlap(a.h, xb, a.x, xb)) return cudaErrorInvalidValue;
-  if (ranges_overlap(a.h, xb, a.o, n * 2) || ranges_overlap(a.h, xb, a.out, yb) ||
-      ranges_overlap(a.out, yb, a.x, xb) || ranges_overlap(a.out, yb, a.o, n * 2))
+  if (a.h && a.h != a.x && detail::ranges_overlap(a.h, xb, a.x, xb)) return cudaErrorInvalidValue;
+  if (detail::ranges_overlap(a.h, xb, a.o, n * 2) || detail::ranges_overlap(a.h, xb, a.out, yb) ||
+      detail::ranges_overlap(a.out, yb, a.x, xb) || detail::ranges_overlap(a.out, yb, a.o, n * 2))
     return cudaErrorInvalidValue;
   return cudaSuccess;
 }
@@ -148,11 +141,11 @@ inline cudaError_t block_norm_backward_check(const blackhole_sm100_block_norm_ba
   }
   const int64_t n = int64_t(a.rows) * a.H;
   const int64_t xb = n * (a.x_is_bf16 ? 2 : 4);
-  if (a.dx != a.dh && ranges_overlap(a.dx, xb, a.dh, xb)) return cudaErrorInvalidValue;
-  if (ranges_overlap(a.dx, xb, a.h, xb) || ranges_overlap(a.dx, xb, a.dy, n * 2) ||
-      ranges_overlap(a.dx, xb, a.o, n * 2) || ranges_overlap(a.dx, xb, a.d_o, n * 2) ||
-      ranges_overlap(a.d_o, n * 2, a.h, xb) || ranges_overlap(a.d_o, n * 2, a.dh, xb) ||
-      ranges_overlap(a.d_o, n * 2, a.dy, n * 2) || ranges_overlap(a.d_o, n * 2, a.o, n * 2))
+  if (a.dx != a.dh && detail::ranges_overlap(a.dx, xb, a.dh, xb)) return cudaErrorInvalidValue;
+  if (detail::ranges_overlap(a.dx, xb, a.h, xb) || detail::ranges_overlap(a.dx, xb, a.dy, n * 2) ||
+      detail::ranges_overlap(a.dx, xb, a.o, n * 2) || detail::ranges_overlap(a.dx, xb, a.d_o, n * 2) ||
+      detail::ranges_overlap(a.d_o, n * 2, a.h, xb) || detail::ranges_overlap(a.d_o, n * 2, a.dh, xb) ||
+      detail::ranges_overlap(a.d_o, n * 2, a.dy, n * 2) || detail::ranges_overlap(a.d_o, n * 2, a.o, n * 2))
     return cudaErrorInvalidValue;
   return cudaSuccess;
 }

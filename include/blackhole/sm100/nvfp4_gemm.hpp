@@ -45,6 +45,7 @@
 #include <blackhole/common/sf_layout.hpp>
 #include <blackhole_sm100.h>
 
+#include <blackhole/sm100/gemm_epilogue.hpp>
 #include <blackhole/sm100/nvfp4_gemm_common.hpp>
 
 #if defined(__CUDACC__)
@@ -100,15 +101,21 @@ inline cudaError_t library_workspace(int dev, cudaStream_t stream, int64_t bytes
 
 // Full control: element format, schedule choice and (for the skinny schedule) a caller-owned
 // workspace.  workspace == nullptr selects the library-owned workspace.
-template <class Fmt>
+// kFused: the result goes through the epilogue `epi` (gemm_epilogue.hpp) on its way to D.
+template <class Fmt, bool kFused = false>
 inline cudaError_t block_scaled_bf16_gemm_ex(int M, int N, int K, void const* A, void const* SFA,
                                              void const* B, void const* SFB, void* D, float alpha,
                                              Nvfp4Schedule schedule, void* workspace,
-                                             int64_t workspace_bytes, cudaStream_t stream) {
+                                             int64_t workspace_bytes, cudaStream_t stream,
+                                             const blackhole_sm100_epilogue* epi = nullptr) {
   cudaError_t e = nvfp4_check_args(M, N, K, A, SFA, B, SFB, D);
   if (e != cudaSuccess) return e;
   e = detail::format_check_args<Fmt>(K, B);
   if (e != cudaSuccess) return e;
+  if constexpr (kFused) {
+    e = epilogue_check_args(M, N, D, epi);
+    if (e != cudaSuccess) return e;
+  }
   detail::DeviceState* st = detail::prepare_device();
   if (!st) return cudaErrorInvalidDevice;
   if (st->init_err != cudaSuccess) return st->init_err;
@@ -121,11 +128,11 @@ inline cudaError_t block_scaled_bf16_gemm_ex(int M, int N, int K, void const* A,
                           : Nvfp4Schedule::kTwoSm;
   switch (schedule) {
     case Nvfp4Schedule::kOneSm:
-      return detail::launch_1sm<Nvfp4GemmTraitsT<4, Fmt>>(M, N, K, A, SFA, B, SFB, D, alpha, st,
-                                                           dev, stream);
+      return detail::launch_1sm<Nvfp4GemmTraitsT<4, Fmt>, kFused>(M, N, K, A, SFA, B, SFB, D, alpha,
+                                                                   st, dev, stream, epi);
     case Nvfp4Schedule::kTwoSm:
-      return detail::launch_2sm<Nvfp4Gemm2SmTraitsT<5, Fmt>>(M, N, K, A, SFA, B, SFB, D, alpha,
-                                                              st, dev, stream);
+      return detail::launch_2sm<Nvfp4Gemm2SmTraitsT<5, Fmt>, kFused>(
+          M, N, K, A, SFA, B, SFB, D, alpha, st, dev, stream, nullptr, epi);
     case Nvfp4Schedule::kSkinny:
     case Nvfp4Schedule::kSkinnyNoPrefetch: {
       if (M > 128) return cudaErrorInvalidValue;
@@ -135,9 +142,9 @@ inline cudaError_t block_scaled_bf16_gemm_ex(int M, int N, int K, void const* A,
         if (e != cudaSuccess) return e;
         workspace_bytes = need;
       }
-      return block_scaled_bf16_gemm_skinny<Fmt>(M, N, K, A, SFA, B, SFB, D, alpha, workspace,
-                                                workspace_bytes, stream, 1 << 30,
-                                                schedule == Nvfp4Schedule::kSkinny);
+      return block_scaled_bf16_gemm_skinny<Fmt, kFused>(
+          M, N, K, A, SFA, B, SFB, D, alpha, workspace, workspace_bytes, stream, 1 << 30,
+          schedule == Nvfp4Schedule::kSkinny, nullptr, ptx::kWaitLimitNs, epi);
     }
     default:
       return cudaErrorInvalidValue;
@@ -178,6 +185,18 @@ inline cudaError_t mxfp4_bf16_gemm(int M, int N, int K, void const* A, void cons
                                    cudaStream_t stream = nullptr) {
   return mxfp4_bf16_gemm_ex(M, N, K, A, SFA, B, SFB, D, alpha, Nvfp4Schedule::kAuto, nullptr, 0,
                             stream);
+}
+
+// The products with bias, activation or gated activation and residual in their epilogue
+// (gemm_epilogue.hpp): shapes, schedules and errors as above, plus N % 16 == 0 when gated.
+template <class Fmt>
+inline cudaError_t block_scaled_bf16_gemm_fused(int M, int N, int K, void const* A, void const* SFA,
+                                                void const* B, void const* SFB, void* D, float alpha,
+                                                const blackhole_sm100_epilogue* epi,
+                                                Nvfp4Schedule schedule, void* workspace,
+                                                int64_t workspace_bytes, cudaStream_t stream) {
+  return block_scaled_bf16_gemm_ex<Fmt, true>(M, N, K, A, SFA, B, SFB, D, alpha, schedule, workspace,
+                                              workspace_bytes, stream, epi);
 }
 
 // GEMM with the output gathered in the same kernel: the M x N result goes to columns

@@ -19,6 +19,7 @@
 // =====================================================================================
 
 #include <blackhole/sm100/block_scale_format.hpp>
+#include <blackhole/sm100/gemm_epilogue.hpp>
 #include <blackhole/sm100/nvfp4_gemm_common.hpp>
 
 namespace blackhole::sm100 {
@@ -105,6 +106,10 @@ struct Nvfp4GemmParams {
   CUtensorMap tmap_sfb; // (sf_tail only) SFB [N/128][atoms][512 B], box 4 atoms x 2 blocks
 };
 
+// The same with an epilogue (its own instantiation: the plain one carries none of its code).
+struct Nvfp4GemmFusedParams : Nvfp4GemmParams {
+  detail::EpilogueParams epi;
+};
 
 namespace detail {
 
@@ -122,9 +127,10 @@ __device__ __forceinline__ void tile_coords(int tile, const Nvfp4GemmParams& p, 
 
 }  // namespace detail
 
-template <class KT>
+template <class KT, bool kFused = false>
 __global__ void __launch_bounds__(KT::NumThreads, 1)
-    nvfp4_gemm_kernel(const __grid_constant__ Nvfp4GemmParams p) {
+    nvfp4_gemm_kernel(const __grid_constant__
+                      std::conditional_t<kFused, Nvfp4GemmFusedParams, Nvfp4GemmParams> p) {
 #if defined(BLACKHOLE_ARCH_SM100)
   using namespace ptx;
   constexpr int S = KT::Stages;
@@ -385,10 +391,54 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
           }
         }
       };
-      stage_store(v0, 0);
-      stage_store(v1, 32);
-      stage_store(v2, 64);
-      stage_store(v3, 96);
+      if constexpr (kFused) {
+        // One 32 x 16 box of bits[0..15] (FP32) to `map` at (row0, col), after adding the
+        // residual when `d`.
+        auto store_box = [&](uint32_t* bits, const CUtensorMap* map, int col, int cols, bool d) {
+          if (lane == 0) bulk_wait_group_read<0>();
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(bits[8 * c + i]);
+            if (d) detail::epilogue_residual8(f, p.epi, row0 + lane, col + 8 * c, p.M);
+            st_shared_v4(my_row + ((c ^ sw) << 4), detail::pack_bf16x2(f[0], f[1]),
+                         detail::pack_bf16x2(f[2], f[3]), detail::pack_bf16x2(f[4], f[5]),
+                         detail::pack_bf16x2(f[6], f[7]));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < p.M && col < cols) {
+            tma_store_2d(map, box, col, row0, pol_d);
+            bulk_commit_group();
+          }
+        };
+        auto finish = [&](uint32_t (&v)[32], int c32) {
+          const int col = col0 + c32;
+          detail::epilogue_z32(v, a, p.epi, col, p.N);
+          if (p.epi.has_z) {
+            store_box(v, &p.epi.tmap_z, col, p.N, false);
+            store_box(v + 16, &p.epi.tmap_z, col + 16, p.N, false);
+          }
+          detail::epilogue_act32(v, p.epi);
+          if (p.epi.gated) {
+            store_box(v, &p.tmap_d, col / 2, p.epi.n_out, true);
+          } else {
+            store_box(v, &p.tmap_d, col, p.N, true);
+            store_box(v + 16, &p.tmap_d, col + 16, p.N, true);
+          }
+        };
+        finish(v0, 0);
+        finish(v1, 32);
+        finish(v2, 64);
+        finish(v3, 96);
+      } else {
+        stage_store(v0, 0);
+        stage_store(v1, 32);
+        stage_store(v2, 64);
+        stage_store(v3, 96);
+      }
     }
     if (lane == 0) bulk_wait_group<0>();
     __syncwarp();
@@ -405,18 +455,24 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
 
 namespace detail {
 
-template <class KT>
+template <class KT, bool kFused = false>
 inline cudaError_t launch_1sm(int M, int N, int K, const void* A, const void* SFA, const void* B,
                               const void* SFB, void* D, float alpha, DeviceState* st, int dev,
-                              cudaStream_t stream) {
-  cudaError_t e = set_smem_once(nvfp4_gemm_kernel<KT>, KT::SmemBytes, dev);
+                              cudaStream_t stream, const blackhole_sm100_epilogue* epi = nullptr) {
+  cudaError_t e = set_smem_once(nvfp4_gemm_kernel<KT, kFused>, KT::SmemBytes, dev);
   if (e != cudaSuccess) return e;
-  Nvfp4GemmParams p;
+  std::conditional_t<kFused, Nvfp4GemmFusedParams, Nvfp4GemmParams> p;
+  int n_out = N;
+  if constexpr (kFused) {
+    e = make_epilogue(&p.epi, *epi, M, N, 16);
+    if (e != cudaSuccess) return e;
+    n_out = p.epi.n_out;
+  }
   e = make_a_tmap<typename KT::Fmt>(&p.tmap_a, A, M, K, KT::TileM);
   if (e != cudaSuccess) return e;
   e = make_b_tmap<typename KT::Fmt>(&p.tmap_b, B, N, K, KT::TileN);
   if (e != cudaSuccess) return e;
-  e = make_d_tmap(&p.tmap_d, D, M, N, 16);
+  e = make_d_tmap(&p.tmap_d, D, M, n_out, 16);
   if (e != cudaSuccess) return e;
   p.sfa = static_cast<const uint8_t*>(SFA);
   p.sfb = static_cast<const uint8_t*>(SFB);
@@ -439,7 +495,7 @@ inline cudaError_t launch_1sm(int M, int N, int K, const void* A, const void* SF
     if (e != cudaSuccess) return e;
   }
   const int grid = p.num_tiles < st->num_sms ? p.num_tiles : st->num_sms;
-  e = launch_pdl(nvfp4_gemm_kernel<KT>, dim3(grid), dim3(KT::NumThreads), KT::SmemBytes, stream, p);
+  e = launch_pdl(nvfp4_gemm_kernel<KT, kFused>, dim3(grid), dim3(KT::NumThreads), KT::SmemBytes, stream, p);
   if (e != cudaSuccess) return e;
   return cudaGetLastError();
 }

@@ -31,6 +31,7 @@
 // =====================================================================================
 
 #include <blackhole/sm100/block_scale_format.hpp>
+#include <blackhole/sm100/gemm_epilogue.hpp>
 #include <blackhole/sm100/nvfp4_gemm_common.hpp>
 
 namespace blackhole::sm100 {
@@ -145,6 +146,11 @@ struct Nvfp4Gemm2SmParams {
   uint8_t* peer_d[kMaxGatherPeers];
 };
 
+// The same with an epilogue (its own instantiation: the plain one carries none of its code).
+struct Nvfp4Gemm2SmFusedParams : Nvfp4Gemm2SmParams {
+  detail::EpilogueParams epi;
+};
+
 namespace detail {
 
 // Tile-rows per raster group: a group's rows of A (and SFA) stay in L2 while every column of B
@@ -179,9 +185,10 @@ __device__ __forceinline__ void tile_coords_2sm(int tile, const Nvfp4Gemm2SmPara
 
 }  // namespace detail
 
-template <class KT, bool kGather = false>
+template <class KT, bool kGather = false, bool kFused = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
-    nvfp4_gemm_2sm_kernel(const __grid_constant__ Nvfp4Gemm2SmParams p) {
+    nvfp4_gemm_2sm_kernel(const __grid_constant__
+                          std::conditional_t<kFused, Nvfp4Gemm2SmFusedParams, Nvfp4Gemm2SmParams> p) {
 #if defined(BLACKHOLE_ARCH_SM100)
   using namespace ptx;
   constexpr int S = KT::Stages;
@@ -600,8 +607,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
           }
         }
       };
-      stage_store(v0, v1, 0);
-      stage_store(v2, v3, 1);
+      if constexpr (kFused) {
+        // One 32 x 64 box to `map` at (row0, col): its 16-byte chunk c holds the FP32 bits
+        // chunk(c)[0..7], plus the residual when `d`.
+        auto store_box = [&](auto chunk, const CUtensorMap* map, int col, int cols, bool d) {
+          if (lane == 0) bulk_wait_group_read<0>();   // previous box has been read out
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t* bits = chunk(c);
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(bits[i]);
+            if (d) detail::epilogue_residual8(f, p.epi, row0 + lane, col + 8 * c, p.M);
+            st_shared_v4(my_row + ((c ^ (lane & 7)) << 4), detail::pack_bf16x2(f[0], f[1]),
+                         detail::pack_bf16x2(f[2], f[3]), detail::pack_bf16x2(f[4], f[5]),
+                         detail::pack_bf16x2(f[6], f[7]));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < p.M && col < cols) {
+            tma_store_2d(map, box, col, row0, pol_d);
+            bulk_commit_group();
+          }
+        };
+        auto chunk01 = [&](int c) -> const uint32_t* { return (c < 4 ? v0 : v1) + 8 * (c & 3); };
+        auto chunk23 = [&](int c) -> const uint32_t* { return (c < 4 ? v2 : v3) + 8 * (c & 3); };
+        detail::epilogue_z32(v0, a, p.epi, col0, p.N);
+        detail::epilogue_z32(v1, a, p.epi, col0 + 32, p.N);
+        detail::epilogue_z32(v2, a, p.epi, col0 + 64, p.N);
+        detail::epilogue_z32(v3, a, p.epi, col0 + 96, p.N);
+        if (p.epi.has_z) {
+          store_box(chunk01, &p.epi.tmap_z, col0, p.N, false);
+          store_box(chunk23, &p.epi.tmap_z, col0 + 64, p.N, false);
+        }
+        detail::epilogue_act32(v0, p.epi);
+        detail::epilogue_act32(v1, p.epi);
+        detail::epilogue_act32(v2, p.epi);
+        detail::epilogue_act32(v3, p.epi);
+        if (p.epi.gated) {
+          auto pairs = [&](int c) -> const uint32_t* {
+            return (c < 2 ? v0 : c < 4 ? v1 : c < 6 ? v2 : v3) + 8 * (c & 1);
+          };
+          store_box(pairs, &p.tmap_d, col0 / 2, p.epi.n_out, true);
+        } else {
+          store_box(chunk01, &p.tmap_d, col0, p.N, true);
+          store_box(chunk23, &p.tmap_d, col0 + 64, p.N, true);
+        }
+      } else {
+        stage_store(v0, v1, 0);
+        stage_store(v2, v3, 1);
+      }
     }
     if (lane == 0) bulk_wait_group<0>();
     __syncwarp();
@@ -619,20 +675,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
 
 namespace detail {
 
-template <class KT>
+template <class KT, bool kFused = false>
 inline cudaError_t launch_2sm(int M, int N, int K, const void* A, const void* SFA, const void* B,
                               const void* SFB, void* D, float alpha, DeviceState* st, int dev,
-                              cudaStream_t stream, const GatherSpec* g = nullptr) {
+                              cudaStream_t stream, const GatherSpec* g = nullptr,
+                              const blackhole_sm100_epilogue* epi = nullptr) {
   // gather mode has its own instantiation (NVFP4 only: the gather entry point's format), so
   // the plain GEMM carries none of its code
   constexpr bool kCanGather = std::is_same_v<typename KT::Fmt, Nvfp4Format>;
   if (g && !kCanGather) return cudaErrorInvalidValue;
-  auto* kernel = nvfp4_gemm_2sm_kernel<KT, false>;
-  if constexpr (kCanGather)
+  auto* kernel = nvfp4_gemm_2sm_kernel<KT, false, kFused>;
+  if constexpr (kCanGather && !kFused)
     if (g) kernel = nvfp4_gemm_2sm_kernel<KT, true>;
   cudaError_t e = set_smem_once(kernel, KT::SmemBytes, dev);
   if (e != cudaSuccess) return e;
-  Nvfp4Gemm2SmParams p;
+  std::conditional_t<kFused, Nvfp4Gemm2SmFusedParams, Nvfp4Gemm2SmParams> p;
+  int n_out = N;
+  if constexpr (kFused) {
+    e = make_epilogue(&p.epi, *epi, M, N, 64);
+    if (e != cudaSuccess) return e;
+    n_out = p.epi.n_out;
+  }
   e = make_a_tmap<typename KT::Fmt>(&p.tmap_a, A, M, K, KT::CtaM);
   if (e != cudaSuccess) return e;
   e = make_b_tmap<typename KT::Fmt>(&p.tmap_b, B, N, K, KT::CtaN);
@@ -655,7 +718,7 @@ inline cudaError_t launch_2sm(int M, int N, int K, const void* A, const void* SF
     for (int i = 0; i < kMaxGatherPeers; ++i)
       p.peer_d[i] = i + 1 < g->ndst ? static_cast<uint8_t*>(g->dst[i + 1]) + g->col0 * 2 : nullptr;
   } else {
-    e = make_d_tmap(&p.tmap_d, D, M, N);
+    e = make_d_tmap(&p.tmap_d, D, M, n_out);
   }
   if (e != cudaSuccess) return e;
   p.status = st->status;

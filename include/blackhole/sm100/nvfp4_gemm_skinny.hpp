@@ -35,6 +35,7 @@
 #include <cstdint>
 
 #include <blackhole/sm100/block_scale_format.hpp>
+#include <blackhole/sm100/gemm_epilogue.hpp>
 #include <blackhole/sm100/nvfp4_gemm_common.hpp>
 
 namespace blackhole::sm100 {
@@ -150,6 +151,10 @@ struct Nvfp4SkinnyParams {
   CUtensorMap tmap_sfw; // (sf_tail only) SFB [N/128][atoms][512 B], box 4 atoms x 1 block
   CUtensorMap tmap_sfx; // (sf_tail only) SFA [1][atoms][512 B], box 4 atoms
 };
+// The same with an epilogue (its own instantiation: the plain one carries none of its code).
+struct Nvfp4SkinnyFusedParams : Nvfp4SkinnyParams {
+  detail::EpilogueParams epi;
+};
 
 namespace skinny_detail {
 
@@ -214,9 +219,10 @@ __device__ __forceinline__ void st_release(uint32_t* p, uint32_t v) {
 
 }  // namespace skinny_detail
 
-template <class KT, bool kGather = false>
+template <class KT, bool kGather = false, bool kFused = false>
 __global__ void __launch_bounds__(KT::NumThreads, 1)
-    nvfp4_gemm_skinny_kernel(const __grid_constant__ Nvfp4SkinnyParams p) {
+    nvfp4_gemm_skinny_kernel(const __grid_constant__
+                             std::conditional_t<kFused, Nvfp4SkinnyFusedParams, Nvfp4SkinnyParams> p) {
 #if defined(BLACKHOLE_ARCH_SM100)
   using namespace ptx;
   using namespace skinny_detail;
@@ -554,17 +560,50 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
         if (sg.kt0 > 0 && !add_partials(sg, v)) break;
       }
       const float a = p.alpha;
+      if constexpr (kFused) {
+        // a lane holds output column n of EC rows; when gated, even lanes hold the gate and the
+        // lane above the up feature of the same column of D
+        const detail::EpilogueParams& ep = p.epi;
+        const bool in = n < p.N;
+        const float bias = in ? detail::epilogue_bias(ep, n) : 0.f;
 #pragma unroll
-      for (int m = 0; m < EC; ++m) {
-        if (m0 + m < p.M && n < p.N) {
-          __nv_bfloat16 b = __float2bfloat16_rn(a * v[m]);
-          const uint16_t bits = *reinterpret_cast<uint16_t*>(&b);
-          // the plain GEMM keeps D's own row stride; gather mode (its own instantiation, so
-          // the plain one carries none of its code) also stores to every further buffer
-          const int64_t off = int64_t(m0 + m) * (kGather ? p.ldd : int64_t(p.N)) + n;
-          p.d[off] = bits;
-          if constexpr (kGather)
-            for (int q = 0; q < p.num_peers; ++q) p.peer_d[q][off] = bits;
+        for (int m = 0; m < EC; ++m) {
+          v[m] = fmaf(a, v[m], bias);
+          if (ep.has_z && in && m0 + m < p.M)
+            ep.z[int64_t(m0 + m) * p.N + n] = static_cast<uint16_t>(detail::pack_bf16x2(v[m], 0.f));
+        }
+        detail::with_activation(ep.activation, [&](auto act) {
+          constexpr int A = decltype(act)::value;
+#pragma unroll
+          for (int m = 0; m < EC; ++m) {
+            const float up = ep.gated ? __shfl_xor_sync(0xFFFFFFFFu, v[m], 1) : 1.f;
+            v[m] = detail::act_value<A>(v[m]);
+            if (ep.gated) v[m] *= up;
+          }
+        });
+        const int nd = ep.gated ? n >> 1 : n;
+        const bool mine = in && !(ep.gated && (n & 1));
+#pragma unroll
+        for (int m = 0; m < EC; ++m) {
+          if (mine && m0 + m < p.M) {
+            const int64_t off = int64_t(m0 + m) * ep.n_out + nd;
+            if (ep.residual) v[m] = fmaf(ep.beta, detail::bf16_value(ep.residual[off]), v[m]);
+            p.d[off] = static_cast<uint16_t>(detail::pack_bf16x2(v[m], 0.f));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int m = 0; m < EC; ++m) {
+          if (m0 + m < p.M && n < p.N) {
+            __nv_bfloat16 b = __float2bfloat16_rn(a * v[m]);
+            const uint16_t bits = *reinterpret_cast<uint16_t*>(&b);
+            // the plain GEMM keeps D's own row stride; gather mode (its own instantiation, so
+            // the plain one carries none of its code) also stores to every further buffer
+            const int64_t off = int64_t(m0 + m) * (kGather ? p.ldd : int64_t(p.N)) + n;
+            p.d[off] = bits;
+            if constexpr (kGather)
+              for (int q = 0; q < p.num_peers; ++q) p.peer_d[q][off] = bits;
+          }
         }
       }
     }
@@ -581,25 +620,30 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
 
 namespace detail {
 
-template <class KT>
+template <class KT, bool kFused = false>
 inline cudaError_t launch_skinny(int M, int N, int K, const void* A, const void* SFA, const void* B,
                                  const void* SFB, void* D, float alpha, void* ws, int64_t ws_bytes,
                                  int grid_cap, bool prefetch, DeviceState* st, cudaStream_t stream,
                                  int l2_prefetch_ktiles = KT::L2PrefetchKTiles,
                                  int skew = KT::RangeSkew, const GatherSpec* g = nullptr,
-                                 uint64_t partial_wait_ns = ptx::kWaitLimitNs) {
+                                 uint64_t partial_wait_ns = ptx::kWaitLimitNs,
+                                 const blackhole_sm100_epilogue* epi = nullptr) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   // gather mode has its own instantiation (NVFP4 only: the gather entry point's format)
   constexpr bool kCanGather = std::is_same_v<typename KT::Fmt, Nvfp4Format>;
   if (g && !kCanGather) return cudaErrorInvalidValue;
-  auto* kernel = nvfp4_gemm_skinny_kernel<KT, false>;
-  if constexpr (kCanGather)
+  auto* kernel = nvfp4_gemm_skinny_kernel<KT, false, kFused>;
+  if constexpr (kCanGather && !kFused)
     if (g) kernel = nvfp4_gemm_skinny_kernel<KT, true>;
   e = set_smem_once(kernel, KT::SmemBytes, dev);
   if (e != cudaSuccess) return e;
-  Nvfp4SkinnyParams p;
+  std::conditional_t<kFused, Nvfp4SkinnyFusedParams, Nvfp4SkinnyParams> p;
+  if constexpr (kFused) {
+    e = make_epilogue(&p.epi, *epi, M, N, 0);
+    if (e != cudaSuccess) return e;
+  }
   e = make_b_tmap<typename KT::Fmt>(&p.tmap_w, B, N, K, 128);
   if (e != cudaSuccess) return e;
   e = make_a_tmap<typename KT::Fmt>(&p.tmap_x, A, M, K, KT::MPAD);
@@ -662,7 +706,7 @@ inline cudaError_t launch_skinny(int M, int N, int K, const void* A, const void*
 // the stream, issues L2 prefetches of the first B / SFB tiles of its range while that kernel
 // is finishing; every load, store and workspace access still waits for its completion, so
 // the results are those of plain stream order either way.
-template <class Fmt = Nvfp4Format>
+template <class Fmt = Nvfp4Format, bool kFused = false>
 inline cudaError_t block_scaled_bf16_gemm_skinny(int M, int N, int K, void const* A,
                                                  void const* SFA, void const* B, void const* SFB,
                                                  void* D, float alpha, void* workspace,
@@ -670,7 +714,8 @@ inline cudaError_t block_scaled_bf16_gemm_skinny(int M, int N, int K, void const
                                                  cudaStream_t stream = nullptr,
                                                  int grid_cap = 1 << 30, bool prefetch = true,
                                                  const detail::GatherSpec* g = nullptr,
-                                                 uint64_t partial_wait_ns = ptx::kWaitLimitNs) {
+                                                 uint64_t partial_wait_ns = ptx::kWaitLimitNs,
+                                                 const blackhole_sm100_epilogue* epi = nullptr) {
   cudaError_t e = nvfp4_check_args(M, N, K, A, SFA, B, SFB, D);
   if (e != cudaSuccess) return e;
   e = detail::format_check_args<Fmt>(K, B);
@@ -682,25 +727,25 @@ inline cudaError_t block_scaled_bf16_gemm_skinny(int M, int N, int K, void const
   if (st->init_err != cudaSuccess) return st->init_err;
   switch (nvfp4_skinny_mpad(M)) {
     case 16:
-      return detail::launch_skinny<Nvfp4SkinnyTraits<16, Fmt>>(
+      return detail::launch_skinny<Nvfp4SkinnyTraits<16, Fmt>, kFused>(
           M, N, K, A, SFA, B, SFB, D, alpha, workspace, workspace_bytes, grid_cap, prefetch, st, stream,
           Nvfp4SkinnyTraits<16, Fmt>::L2PrefetchKTiles, Nvfp4SkinnyTraits<16, Fmt>::RangeSkew, g,
-          partial_wait_ns);
+          partial_wait_ns, epi);
     case 32:
-      return detail::launch_skinny<Nvfp4SkinnyTraits<32, Fmt>>(
+      return detail::launch_skinny<Nvfp4SkinnyTraits<32, Fmt>, kFused>(
           M, N, K, A, SFA, B, SFB, D, alpha, workspace, workspace_bytes, grid_cap, prefetch, st, stream,
           Nvfp4SkinnyTraits<32, Fmt>::L2PrefetchKTiles, Nvfp4SkinnyTraits<32, Fmt>::RangeSkew, g,
-          partial_wait_ns);
+          partial_wait_ns, epi);
     case 64:
-      return detail::launch_skinny<Nvfp4SkinnyTraits<64, Fmt>>(
+      return detail::launch_skinny<Nvfp4SkinnyTraits<64, Fmt>, kFused>(
           M, N, K, A, SFA, B, SFB, D, alpha, workspace, workspace_bytes, grid_cap, prefetch, st, stream,
           Nvfp4SkinnyTraits<64, Fmt>::L2PrefetchKTiles, Nvfp4SkinnyTraits<64, Fmt>::RangeSkew, g,
-          partial_wait_ns);
+          partial_wait_ns, epi);
     default:
-      return detail::launch_skinny<Nvfp4SkinnyTraits<128, Fmt>>(
+      return detail::launch_skinny<Nvfp4SkinnyTraits<128, Fmt>, kFused>(
           M, N, K, A, SFA, B, SFB, D, alpha, workspace, workspace_bytes, grid_cap, prefetch, st, stream,
           Nvfp4SkinnyTraits<128, Fmt>::L2PrefetchKTiles, Nvfp4SkinnyTraits<128, Fmt>::RangeSkew, g,
-          partial_wait_ns);
+          partial_wait_ns, epi);
   }
 }
 

@@ -221,6 +221,56 @@ BLACKHOLE_SM100_API int blackhole_sm100_mxfp4_quantize(const void* X, int x_is_b
                                                        int K, void* packed, void* sf,
                                                        cudaStream_t stream);
 
+/* The products with an epilogue fused into them (no counterpart in the reference):
+ *     z = alpha * A . B^T + bias                                              (FP32)
+ *     u = act(z), or gated (N % 16 == 0): u[:, j] = act(z[:, 2j]) * z[:, 2j + 1], N / 2 columns
+ *     D = bf16(u + beta * residual)
+ * for the three operand formats; all other arguments, shapes, schedules and errors as the _ex
+ * calls.  Gate and up features alternate: gate row j of the weights is row 2j of B, up row j
+ * row 2j + 1 (and so in SFB and bias).
+ *   activation : 0 none, 1 ReLU, 2 GELU (erf), 3 GELU (tanh), 4 SiLU
+ *   bias       : N values, BF16 (bias_is_bf16) or FP32, or NULL
+ *   residual   : BF16 of D's shape (M x N, gated M x N / 2), or NULL; may be D itself
+ *   Z          : BF16 M x N, receives z for the backward pass, or NULL
+ * bias, residual and Z 16-byte aligned; Z and residual do not overlap D otherwise.  One library
+ * workspace per (device, stream) serves the skinny schedule as in the _ex calls: graphs captured
+ * on one stream that may replay at once pass workspaces of their own. */
+typedef struct blackhole_sm100_epilogue {
+  int activation, gated, bias_is_bf16;
+  float beta;
+  const void *bias, *residual;
+  void* Z;
+} blackhole_sm100_epilogue;
+BLACKHOLE_SM100_API int blackhole_sm100_nvfp4_bf16_gemm_fused(
+    int M, int N, int K, const void* A, const void* SFA, const void* B, const void* SFB, void* D,
+    float alpha, const blackhole_sm100_epilogue* epilogue, int schedule, void* workspace,
+    int64_t workspace_bytes, cudaStream_t stream);
+BLACKHOLE_SM100_API int blackhole_sm100_mxfp4_bf16_gemm_fused(
+    int M, int N, int K, const void* A, const void* SFA, const void* B, const void* SFB, void* D,
+    float alpha, const blackhole_sm100_epilogue* epilogue, int schedule, void* workspace,
+    int64_t workspace_bytes, cudaStream_t stream);
+BLACKHOLE_SM100_API int blackhole_sm100_mxf8f4_bf16_gemm_fused(
+    int M, int N, int K, const void* A, const void* SFA, const void* B, const void* SFB, void* D,
+    float alpha, const blackhole_sm100_epilogue* epilogue, int schedule, void* workspace,
+    int64_t workspace_bytes, cudaStream_t stream);
+
+/* Gradient through that epilogue, from the Z it kept:  dZ = dD * act'(Z), or gated
+ * dZ[:, 2j] = dD[:, j] act'(Z[:, 2j]) Z[:, 2j + 1] and dZ[:, 2j + 1] = dD[:, j] act(Z[:, 2j]);
+ * dbias = column sums of dZ before its rounding.  (The residual's gradient is beta * dD, those of
+ * the operands are products with alpha * dZ.)
+ *   dD, Z, dZ : BF16, M x N (dD gated M x N / 2); dZ may be Z, or dD when not gated
+ *   dbias     : N FP32 values (overwritten), or NULL
+ *   workspace : blackhole_sm100_gemm_fused_backward_workspace_bytes(M, N) bytes for dbias's sums
+ *               (NULL without dbias or where that is 0); contents do not matter; calls sharing one
+ *               must be ordered, replays of captured graphs among them
+ * M >= 1, N % 8 == 0 (gated 16), 16-byte aligned.  dbias is summed in an order fixed by M and N. */
+BLACKHOLE_SM100_API int blackhole_sm100_gemm_fused_backward(int M, int N, const void* dD, const void* Z,
+                                                            void* dZ, float* dbias, int activation,
+                                                            int gated, void* workspace,
+                                                            int64_t workspace_bytes,
+                                                            cudaStream_t stream);
+BLACKHOLE_SM100_API int64_t blackhole_sm100_gemm_fused_backward_workspace_bytes(int M, int N);
+
 /* Norms before and after a block, fused with its gate and residual scale (no counterpart in the
  * reference): per row of H features
  *     p = o, or norm(o) * post_weight + post_bias with post_norm
