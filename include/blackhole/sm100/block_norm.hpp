@@ -23,7 +23,10 @@
 // ([...]: layer norm only).
 //
 // A row is worked on by one CTA (H <= 8192) or a cluster of two (H <= 16384), 16 columns per
-// thread as two 8-column vectors.
+// thread as two 8-column vectors; CTAs are persistent, each over a range of consecutive rows.  Rows
+// arrive in shared memory through a ring of bulk copies that runs ahead of the arithmetic, so that
+// HBM keeps streaming through the row sums' barriers; the parameter vectors, with gate, scale and
+// post weight multiplied into one, stay in registers from row to row.
 // =====================================================================================
 
 #include <algorithm>
@@ -61,28 +64,34 @@ inline Geometry geometry(int H) {
   return g;
 }
 
-// Row ranges of the backward kernel: `teams` CTAs (or clusters) of `rows_per_team` consecutive
-// rows.  Fixed by the sizes alone (148 SMs, 512 resident threads on each), so the workspace size
-// and the order of the column sums do not depend on the device's state.
-struct Teams {
-  int teams;
-  int rows_per_team;
-};
-inline Teams backward_teams(int rows, int H) {
-  const Geometry g = geometry(H);
+// Row ranges: `teams` CTAs (or clusters), each of rows [row_begin(t), row_begin(t + 1)), as many
+// as are resident at once (512 threads of 128 registers per SM, 148 SMs).  Fixed by the sizes
+// alone, so the workspace size and the order of the column sums do not depend on the device.
+inline int row_teams(int rows, const Geometry& g) {
   const int per_sm = std::max(1, 512 / g.threads);
-  const int cap = std::max(1, 148 * per_sm / g.cluster);
-  Teams t;
-  t.rows_per_team = (rows + cap - 1) / cap;
-  t.teams = (rows + t.rows_per_team - 1) / t.rows_per_team;
-  return t;
+  return std::min(rows, std::max(1, 148 * per_sm / g.cluster));
+}
+BLACKHOLE_HD inline int64_t row_begin(int64_t team, int64_t rows, int64_t teams) {
+  return team * rows / teams;
+}
+// The team whose range holds `row`.
+BLACKHOLE_HD inline int64_t team_of(int64_t row, int64_t rows, int64_t teams) {
+  return ((row + 1) * teams - 1) / rows;
+}
+
+// Ring of row stages in shared memory: as many as fit the CTA's share of the SM, 8 at most.
+constexpr int kRingBytesPerSm = 192 * 1024;
+constexpr int kMaxStages = 8;
+inline int ring_stages(const Geometry& g, int stage_bytes, int rows_per_team) {
+  const int share = kRingBytesPerSm / std::max(1, 512 / g.threads);
+  return std::max(1, std::min({share / stage_bytes, kMaxStages, rows_per_team}));
 }
 
 }  // namespace norm_detail
 
 inline int64_t block_norm_backward_workspace_bytes(int rows, int H, int has_gate, int gate_rows) {
   if (rows < 1 || H < 8 || H > kNormMaxH || H % 8 != 0 || gate_rows < 0) return -1;
-  const int64_t teams = norm_detail::backward_teams(rows, H).teams;
+  const int64_t teams = norm_detail::row_teams(rows, norm_detail::geometry(H));
   const int64_t vectors = 4 + ((has_gate && gate_rows != 1) ? 2 : 0);
   return teams * vectors * H * 4;
 }
@@ -173,72 +182,225 @@ __device__ __forceinline__ void load8_any(const void* p, int64_t at, int is_bf16
   if (is_bf16) load8(static_cast<const __nv_bfloat16*>(p) + at, v);
   else load8(static_cast<const float*>(p) + at, v);
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) =
-      make_uint4(detail::pack_bf16x2(v[0], v[1]), detail::pack_bf16x2(v[2], v[3]),
-                 detail::pack_bf16x2(v[4], v[5]), detail::pack_bf16x2(v[6], v[7]));
-}
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
 }
 
-// Sums over the threads of a row's CTA or cluster, the same value in every thread, added in a
-// fixed order.  Two slot sets in turn: a set is written again only after a later barrier that
-// every reader of it has passed.
-template <int kCl, int kN>
-struct RowSum {
-  float (*slots)[kN][kCl * 16];   // [2][kN][CTA * 16 + warp], zeroed before first use
+// Exchange of one pair of values per warp across a row's CTA or cluster.  Two slot sets in turn: a
+// set is written again only after a later barrier that every reader of it has passed.
+template <int kCl>
+struct RowExchange {
+  static constexpr int kWarps = kCl * 16;
+  float (*slots)[2][kWarps];      // [2][2][CTA * 16 + warp], zeroed before first use
+  const float* counts;            // [CTA * 16 + warp]: columns of the row that the warp holds
   int set = 0;
 
-  __device__ __forceinline__ void operator()(float (&v)[kN]) {
+  __device__ __forceinline__ void put(float a, float b) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-    for (int k = 0; k < kN; ++k) v[k] = warp_sum(v[k]);
-    if (kCl == 1 && blockDim.x == 32) return;
     if constexpr (kCl == 1) {
-      if (lane == 0)
-#pragma unroll
-        for (int k = 0; k < kN; ++k) slots[set][k][warp] = v[k];
+      if (lane == 0) {
+        slots[set][0][warp] = a;
+        slots[set][1][warp] = b;
+      }
       __syncthreads();
     } else {
-      const int rank = static_cast<int>(ptx::cluster_ctarank());
-      if (lane < kCl)
+      const uint32_t rank = ptx::cluster_ctarank();
+      if (lane < kCl) {
+        const float v[2] = {a, b};
 #pragma unroll
-        for (int k = 0; k < kN; ++k) {
-          const uint32_t a = ptx::mapa_shared(
-              ptx::smem_u32(&slots[set][k][rank * 16 + warp]), static_cast<uint32_t>(lane));
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v[k]) : "memory");
-        }
+        for (int k = 0; k < 2; ++k)
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(ptx::mapa_shared(
+                           ptx::smem_u32(&slots[set][k][rank * 16 + warp]), uint32_t(lane))),
+                       "f"(v[k])
+                       : "memory");
+      }
       ptx::cluster_sync();
     }
+  }
+  __device__ __forceinline__ float total(int k) const {
+    float s = 0.f;
+    const float4* q = reinterpret_cast<const float4*>(slots[set][k]);
 #pragma unroll
-    for (int k = 0; k < kN; ++k) {
-      float s = 0.f;
-      const float4* q = reinterpret_cast<const float4*>(slots[set][k]);
-#pragma unroll
-      for (int i = 0; i < kCl * 4; ++i) {
-        const float4 t = q[i];
-        s += (t.x + t.y) + (t.z + t.w);
-      }
-      v[k] = s;
+    for (int i = 0; i < kWarps / 4; ++i) {
+      const float4 t = q[i];
+      s += (t.x + t.y) + (t.z + t.w);
     }
+    return s;
+  }
+  // Sums of a and b over the row, the same in every thread, added in a fixed order.  A barrier
+  // of the CTA or cluster, unless the CTA is one warp.
+  __device__ __forceinline__ void sum2(float& a, float& b, bool with_b) {
+    a = warp_sum(a);
+    if (with_b) b = warp_sum(b);
+    if (kCl == 1 && blockDim.x == 32) return;
+    put(a, b);
+    a = total(0);
+    if (with_b) b = total(1);
+    set ^= 1;
+  }
+  // Mean and sum of squares about it of the row's values (16 per thread): each warp's own mean
+  // and squares about that first, then merged, so nothing cancels however far the mean is from
+  // zero, and one barrier is enough.
+  __device__ __forceinline__ void mean_squares(const float (&v)[16], const bool (&live)[2], float inv_h,
+                                               float& mean, float& squares) {
+    const int me = (kCl == 1 ? 0 : int(ptx::cluster_ctarank())) * 16 + (threadIdx.x >> 5);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += v[i];
+    const float n = counts[me];
+    const float mw = n > 0.f ? warp_sum(s) / n : 0.f;
+    float m2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float d = v[i] - mw;
+      m2 += live[i / 8] ? d * d : 0.f;
+    }
+    m2 = warp_sum(m2);
+    if (kCl == 1 && blockDim.x == 32) {
+      mean = mw;
+      squares = m2;
+      return;
+    }
+    put(mw, m2);
+    float total_mean = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) total_mean = fmaf(counts[i], slots[set][0][i], total_mean);
+    total_mean *= inv_h;
+    float q = total(1);
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const float d = slots[set][0][i] - total_mean;
+      q = fmaf(counts[i] * d, d, q);
+    }
+    mean = total_mean;
+    squares = q;
     set ^= 1;
   }
 };
+
+// Shared memory of a CTA: the ring's stages first (dynamic), then this.
+template <int kCl>
+struct __align__(16) RowShared {
+  float slots[2][2][kCl * 16];
+  float counts[kCl * 16];
+  uint64_t bars[kMaxStages];
+  int abort_flag;
+};
+
+// This thread's columns and the CTA's set-up, the same in both directions.
+template <int kCl>
+struct RowTeam {
+  int rank, team, col[2];
+  bool live[2];
+  int64_t row0, row1;
+  int c0, cols;                  // the CTA's columns of a row
+  uint32_t ring, bars;
+  volatile int* abort_flag;
+
+  __device__ __forceinline__ RowTeam(RowShared<kCl>& sh, uint8_t* ring_ptr, int H, int slice, int rows,
+                                     int teams, int stages) {
+    rank = kCl == 1 ? 0 : static_cast<int>(ptx::cluster_ctarank());
+    team = blockIdx.x / kCl;
+    const int T = blockDim.x, tid = threadIdx.x;
+    c0 = rank * slice;
+    const int c1 = min(H, c0 + slice);
+    cols = c1 - c0;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      col[v] = c0 + (v * T + tid) * 8;
+      live[v] = col[v] < c1;
+    }
+    row0 = row_begin(team, rows, teams);
+    row1 = row_begin(team + 1, rows, teams);
+    ring = ptx::smem_u32(ring_ptr);
+    bars = ptx::smem_u32(sh.bars);
+    abort_flag = &sh.abort_flag;
+    for (int i = tid; i < 4 * kCl * 16; i += T) (&sh.slots[0][0][0])[i] = 0.f;
+    for (int i = tid; i < kCl * 16; i += T) {       // columns of warp i % 16 of CTA i / 16
+      const int b = (i / 16) * slice, e = min(H, b + slice);
+      int n = 0;
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int from = b + (v * T + (i % 16) * 32) * 8;
+        if ((i % 16) * 32 < T) n += max(0, min(e, from + 256) - from);
+      }
+      sh.counts[i] = static_cast<float>(n);
+    }
+    if (tid == 0) {
+      for (int s = 0; s < stages; ++s) ptx::mbar_init(bars + 8u * s, 1);
+      sh.abort_flag = 0;
+      ptx::fence_mbar_init();
+      ptx::fence_proxy_async_smem();
+    }
+    if constexpr (kCl == 1) __syncthreads();
+    else ptx::cluster_sync();
+  }
+  // A stage's rows have arrived (bounded like every wait: a copy that never lands sets the status
+  // word, and the kernel runs to its end).
+  __device__ __forceinline__ void wait(int stage, uint32_t phase) {
+    (void)ptx::wait_bounded(bars + 8u * stage, phase, abort_flag, &detail::g_status, kStatusLoadTimeout);
+  }
+  // Every thread of the CTA has read the stage.
+  __device__ __forceinline__ void release_barrier() const { __syncthreads(); }
+};
+
+__device__ __forceinline__ uint4 lds16(uint32_t a) { return ptx::ld_shared_v4(a); }
+__device__ __forceinline__ void unpack8(const uint4& q, float* v) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+// 8 values at element `at` of a row in shared memory.
+template <class T>
+__device__ __forceinline__ void shared8(uint32_t row, int at, float* v) {
+  if constexpr (sizeof(T) == 2) {
+    unpack8(lds16(row + 2 * at), v);
+  } else {
+    const uint4 a = lds16(row + 4 * at), b = lds16(row + 4 * at + 16);
+    v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+    v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float* v) {
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(detail::pack_bf16x2(v[0], v[1]), detail::pack_bf16x2(v[2], v[3]),
+                   detail::pack_bf16x2(v[4], v[5]), detail::pack_bf16x2(v[6], v[7]));
+  } else {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+// This thread's 16 values of a parameter vector (BF16 or FP32), `none` where it is absent.
+__device__ __forceinline__ void vector16(const void* p, int64_t at, int is_bf16, const int (&col)[2],
+                                         const bool (&live)[2], float none, float (&out)[16]) {
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = none;
+    if (p && live[v]) load8_any(p, at + col[v], is_bf16, t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[8 * v + i] = t[i];
+  }
+}
+
+// What a kernel is built for: RMS norms, RMS norms with a bias (or its gradient) somewhere, layer
+// norms.
+enum NormMode : int { kRms = 0, kRmsBias = 1, kLayerNorm = 2 };
 
 struct NormParams {
   const void *x, *o, *gate, *weight, *bias, *post_weight, *post_bias;
   void *h, *out;
   uint8_t* sf;
   float* stats;
-  int rows, H, slice, teams;
+  int rows, H, slice, teams, stages;
   int gate_rows, param_bf16, gate_bf16, out_format;
   float scale, eps, global_scale;
 };
@@ -247,7 +409,7 @@ struct NormParams {
 // columns of the 16- or 32-column block.  Every lane of the warp calls it (`live` false: past
 // the row's end, all zero).  Recipes and roundings are those of nvfp4_quant.hpp.
 template <class Store32, class Store64>
-__device__ __forceinline__ uint32_t quantize8(const float (&y)[8], bool live, int fmt, float g,
+__device__ __forceinline__ uint32_t quantize8(const float* y, bool live, int fmt, float g,
                                               Store32 store32, Store64 store64) {
   float m = 0.f;
 #pragma unroll
@@ -290,166 +452,180 @@ __device__ __forceinline__ uint32_t quantize8(const float (&y)[8], bool live, in
   return code;
 }
 
-template <class TX, bool kLayer, bool kPost, int kCl>
-__global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512)
+// Forward.  kPost and p.o select what a row's p is made of; the gate row, the scale and the post
+// weight are one vector `cw` (and with the post bias `cb`), made anew only where the gate row
+// changes.
+template <class TX, int kMode, bool kPost, int kCl>
+__global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
     block_norm_kernel(const __grid_constant__ NormParams p) {
 #if defined(BLACKHOLE_ARCH_SM100)
-  __shared__ __align__(16) float slots[2][1][kCl * 16];
-  const int rank = kCl == 1 ? 0 : static_cast<int>(ptx::cluster_ctarank());
-  const int team = blockIdx.x / kCl;
-  const int T = blockDim.x, tid = threadIdx.x, lane = tid & 31;
-  const int H = p.H;
-  const int c0 = rank * p.slice, c1 = min(H, c0 + p.slice);
+  constexpr bool kLayer = kMode == kLayerNorm, kBias = kMode != kRms;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ RowShared<kCl> sh;
   ptx::pdl_launch_dependents();
-  for (int i = tid; i < 2 * kCl * 16; i += T) (&slots[0][0][0])[i] = 0.f;
-  if constexpr (kCl == 1) __syncthreads();
-  else ptx::cluster_sync();
-  RowSum<kCl, 1> row_sum{slots};
-  auto sum = [&](float v) {
-    float a[1] = {v};
-    row_sum(a);
-    return a[0];
-  };
+  RowTeam<kCl> t(sh, ring, p.H, p.slice, p.rows, p.teams, p.stages);
+  RowExchange<kCl> row{sh.slots, sh.counts};
+  const int tid = threadIdx.x, lane = tid & 31, H = p.H;
+  const uint32_t x_bytes = uint32_t(t.cols) * sizeof(TX), o_bytes = p.o ? uint32_t(t.cols) * 2 : 0;
+  const uint32_t stage_bytes = uint32_t(p.slice) * (sizeof(TX) + (p.o ? 2 : 0));
   ptx::pdl_wait_prior_grid();
 
-  int col[2];
-  bool live[2];
-#pragma unroll
-  for (int v = 0; v < 2; ++v) {
-    col[v] = c0 + (v * T + tid) * 8;
-    live[v] = col[v] < c1;
-  }
+  const uint64_t policy = ptx::l2_policy_evict_first();   // every row is read once
+  auto fetch = [&](int64_t r, int stage) {
+    const uint32_t bar = t.bars + 8u * stage, dst = t.ring + stage * stage_bytes;
+    ptx::mbar_arrive_expect_tx(bar, x_bytes + o_bytes);
+    ptx::bulk_load(dst, static_cast<const TX*>(p.x) + r * H + t.c0, x_bytes, bar, policy);
+    if (o_bytes)
+      ptx::bulk_load(dst + uint32_t(p.slice) * sizeof(TX),
+                     static_cast<const __nv_bfloat16*>(p.o) + r * H + t.c0, o_bytes, bar, policy);
+  };
+  if (tid == 0)
+    for (int i = 0; i < p.stages && t.row0 + i < t.row1; ++i) fetch(t.row0 + i, i);
+
+  float w[16], b[kBias ? 16 : 1], cw[16], cb[kBias && kPost ? 16 : 1];
+  vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
+  if constexpr (kBias) vector16(p.bias, 0, p.param_bf16, t.col, t.live, 0.f, b);
+  int64_t gate_row = -1;
   const float inv_h = 1.0f / static_cast<float>(H);
-  for (int row = team; row < p.rows; row += p.teams) {
-    const int64_t at = int64_t(row) * H;
-    float h[2][8], mean_post = 0.f, rstd_post = 0.f;
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int64_t r = t.row0; r < t.row1; ++r) {
+    const int64_t at = r * H;
+    const int64_t g = p.gate_rows ? r / p.gate_rows : 0;
+    if (p.o && g != gate_row) {
+      gate_row = g;
+      vector16(p.gate, g * H, p.gate_bf16, t.col, t.live, 1.f, cw);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) cw[i] *= p.scale;
+      if constexpr (kPost) {
+        float v[16];
+        if constexpr (kBias) {
+          vector16(p.post_bias, 0, p.param_bf16, t.col, t.live, 0.f, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) cb[i] = cw[i] * v[i];
+        }
+        vector16(p.post_weight, 0, p.param_bf16, t.col, t.live, 1.f, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) cw[i] *= v[i];
+      }
+    }
+    const uint32_t xs = t.ring + stage * stage_bytes, os = xs + uint32_t(p.slice) * sizeof(TX);
+    t.wait(stage, phase);
+    float h[16], o[16], mean_post = 0.f, rstd_post = 0.f;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[v][i] = 0.f;
-      if (live[v]) load8(static_cast<const TX*>(p.x) + at + col[v], h[v]);
+      for (int i = 0; i < 8; ++i) h[8 * v + i] = o[8 * v + i] = 0.f;
+      if (t.live[v]) {
+        shared8<TX>(xs, t.col[v] - t.c0, h + 8 * v);
+        if (p.o) shared8<__nv_bfloat16>(os, t.col[v] - t.c0, o + 8 * v);
+      }
+    }
+    // every path below meets a barrier of the CTA after these reads, before the refill
+    auto refill = [&]() {
+      if (tid == 0 && r + p.stages < t.row1) fetch(r + p.stages, stage);
+    };
+    if (kPost) {
+      float q = 0.f;
+      if constexpr (kLayer) {
+        row.mean_squares(o, t.live, inv_h, mean_post, q);
+      } else {
+        float none = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) q = fmaf(o[i], o[i], q);
+        row.sum2(q, none, false);
+      }
+      rstd_post = __frsqrt_rn(fmaf(q, inv_h, p.eps));
+      if (blockDim.x == 32) __syncwarp();
+      refill();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = t.live[i / 8] ? (o[i] - mean_post) * rstd_post : 0.f;
     }
     if (p.o) {
-      float o[2][8];
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
+      for (int i = 0; i < 16; ++i) h[i] = fmaf(o[i], cw[i], h[i]);
+      if constexpr (kBias && kPost) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[v][i] = 0.f;
-        if (live[v]) load8(static_cast<const __nv_bfloat16*>(p.o) + at + col[v], o[v]);
+        for (int i = 0; i < 16; ++i) h[i] += cb[i];
       }
-      if constexpr (kPost) {
-        float s = 0.f;
-        if constexpr (kLayer) {
+      if (p.h)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s += o[i / 8][i % 8];
-          mean_post = sum(s) * inv_h;
-        }
-        s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float d = o[i / 8][i % 8] - mean_post;
-          s += live[i / 8] ? d * d : 0.f;
-        }
-        rstd_post = __frsqrt_rn(sum(s) * inv_h + p.eps);
-      }
-      const int64_t gate_at = p.gate_rows ? int64_t(row / p.gate_rows) * H : 0;
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        if (!live[v]) continue;
-        if constexpr (kPost) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[v][i] = (o[v][i] - mean_post) * rstd_post;
-          if (p.post_weight) {
-            float w[8];
-            load8_any(p.post_weight, col[v], p.param_bf16, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[v][i] *= w[i];
-          }
-          if (p.post_bias) {
-            float w[8];
-            load8_any(p.post_bias, col[v], p.param_bf16, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[v][i] += w[i];
-          }
-        }
-        if (p.gate) {
-          float w[8];
-          load8_any(p.gate, gate_at + col[v], p.gate_bf16, w);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[v][i] *= w[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[v][i] = fmaf(p.scale, o[v][i], h[v][i]);
-        if (p.h) store8(static_cast<TX*>(p.h) + at + col[v], h[v]);
-      }
+        for (int v = 0; v < 2; ++v)
+          if (t.live[v]) store8(static_cast<TX*>(p.h) + at + t.col[v], h + 8 * v);
     }
-    if (!p.out && !p.stats) continue;
-    float mean = 0.f, s = 0.f;
-    if constexpr (kLayer) {
+    if (p.out || p.stats) {
+      float mean = 0.f, q = 0.f;
+      if constexpr (kLayer) {
+        row.mean_squares(h, t.live, inv_h, mean, q);
+      } else {
+        float none = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s += h[i / 8][i % 8];
-      mean = sum(s) * inv_h;
-    }
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float d = h[i / 8][i % 8] - mean;
-      s += live[i / 8] ? d * d : 0.f;
-    }
-    const float rstd = __frsqrt_rn(sum(s) * inv_h + p.eps);
-    if (p.stats && rank == 0 && tid == 0)
-      reinterpret_cast<float4*>(p.stats)[row] = make_float4(mean_post, rstd_post, mean, rstd);
-    if (!p.out) continue;
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = live[v] ? (h[v][i] - mean) * rstd : 0.f;
-      if (live[v] && p.weight) {
-        float w[8];
-        load8_any(p.weight, col[v], p.param_bf16, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] *= w[i];
+        for (int i = 0; i < 16; ++i) q = fmaf(h[i], h[i], q);
+        row.sum2(q, none, false);
       }
-      if (live[v] && p.bias) {
-        float w[8];
-        load8_any(p.bias, col[v], p.param_bf16, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] += w[i];
+      if (!kPost) {
+        if (blockDim.x == 32) __syncwarp();
+        refill();
       }
+      const float rstd = __frsqrt_rn(fmaf(q, inv_h, p.eps));
+      if (p.stats && t.rank == 0 && tid == 0)
+        reinterpret_cast<float4*>(p.stats)[r] = make_float4(mean_post, rstd_post, mean, rstd);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) h[i] = t.live[i / 8] ? (h[i] - mean) * rstd * w[i] : 0.f;
+      if constexpr (kBias) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) h[i] += t.live[i / 8] ? b[i] : 0.f;
+      }
+    } else if (!kPost) {
+      t.release_barrier();
+      refill();
+    }
+    if (p.out) {
       if (p.out_format == kOutBf16) {
-        if (live[v]) store8(static_cast<__nv_bfloat16*>(p.out) + at + col[v], y);
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+          if (t.live[v]) store8(static_cast<__nv_bfloat16*>(p.out) + at + t.col[v], h + 8 * v);
       } else if (p.out_format == kOutF32) {
-        if (live[v]) store8(static_cast<float*>(p.out) + at + col[v], y);
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+          if (t.live[v]) store8(static_cast<float*>(p.out) + at + t.col[v], h + 8 * v);
       } else {
         uint8_t* const out = static_cast<uint8_t*>(p.out);
-        const uint32_t code = quantize8(
-            y, live[v], p.out_format, p.global_scale,
-            [&](uint32_t q) {
-              if (live[v]) *reinterpret_cast<uint32_t*>(out + (at + col[v]) / 2) = q;
-            },
-            [&](uint2 q) {
-              if (live[v]) *reinterpret_cast<uint2*>(out + at + col[v]) = q;
-            });
-        // four groups' codes make one word of the row: 2 (NVFP4) or 4 lanes per group
-        const int per = p.out_format == kOutNvfp4 ? 2 : 4;
-        uint32_t word = code << (8 * ((lane / per) & 3));
-        word = (lane % per) == 0 ? word : 0u;
-        for (int o = 4 * per / 2; o > 0; o >>= 1) word |= __shfl_xor_sync(0xFFFFFFFFu, word, o);
-        if ((lane & (4 * per - 1)) == 0 && col[v] < c1)
-          *reinterpret_cast<uint32_t*>(
-              p.sf + sf_offset_vs(row, col[v] / (8 * per), H, 8 * per)) = word;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const uint32_t code = quantize8(
+              h + 8 * v, t.live[v], p.out_format, p.global_scale,
+              [&](uint32_t q) {
+                if (t.live[v]) *reinterpret_cast<uint32_t*>(out + (at + t.col[v]) / 2) = q;
+              },
+              [&](uint2 q) {
+                if (t.live[v]) *reinterpret_cast<uint2*>(out + at + t.col[v]) = q;
+              });
+          // four groups' codes make one word of the row: 2 (NVFP4) or 4 lanes per group
+          const int per = p.out_format == kOutNvfp4 ? 2 : 4;
+          uint32_t word = code << (8 * ((lane / per) & 3));
+          word = (lane % per) == 0 ? word : 0u;
+          for (int k = 4 * per / 2; k > 0; k >>= 1) word |= __shfl_xor_sync(0xFFFFFFFFu, word, k);
+          if ((lane & (4 * per - 1)) == 0 && t.live[v])
+            *reinterpret_cast<uint32_t*>(
+                p.sf + sf_offset_vs(r, t.col[v] / (8 * per), H, 8 * per)) = word;
+        }
       }
+    }
+    if (++stage == p.stages) {
+      stage = 0;
+      phase ^= 1u;
     }
   }
   // scale factors of the layout's padding rows
-  if (p.out && p.sf && rank == 0) {
+  if (p.out && p.sf && t.rank == 0) {
     const int vs = p.out_format == kOutNvfp4 ? 16 : 32;
     const int words = static_cast<int>(sf_k_atoms_vs(H, vs));
     const int pad = (p.rows + 127) / 128 * 128 - p.rows;
-    for (int64_t i = int64_t(team) * T + tid; i < int64_t(pad) * words; i += int64_t(p.teams) * T)
+    for (int64_t i = int64_t(t.team) * blockDim.x + tid; i < int64_t(pad) * words;
+         i += int64_t(p.teams) * blockDim.x)
       *reinterpret_cast<uint32_t*>(
-          p.sf + sf_offset_vs(p.rows + int(i / words), 4 * (i % words), H, vs)) = 0u;
+          p.sf + sf_offset_vs(p.rows + int64_t(i / words), 4 * (i % words), H, vs)) = 0u;
   }
   if constexpr (kCl > 1) ptx::cluster_sync();   // no CTA leaves while its partner writes its slots
 #endif
@@ -461,198 +637,265 @@ struct NormBackwardParams {
   void *dx, *d_o;
   float *dweight, *dbias, *dpost_weight, *dpost_bias, *dgate;
   float* ws;            // [vector][team][H]: dweight, dbias, dpost_weight, dpost_bias, gate edges
-  int rows, H, slice, teams, rows_per_team;
-  int gate_rows, param_bf16, gate_bf16;
+  int rows, H, slice, teams, stages;
+  int gate_rows, groups, param_bf16, gate_bf16;
   float scale;
 };
 
-template <class TX, bool kLayer, bool kPost, bool kGate, int kCl>
+// Backward.  With n the post-normed o (o itself without a post norm) and d = dh', a gate row's
+// sums A = sum d n and B = sum d give every gradient that the gate takes part in:
+//     dgate = scale (post_weight A + post_bias B),  dpost_weight = scale gate A, dpost_bias = scale gate B
+// so a thread keeps dweight, A (and for layer norms dbias, B) for its 16 columns, and gate, scale
+// and post weight are one vector c.  kGate: 0 no gate, 1 one gate row (sums closed once, at the
+// end), 2 several (closed at each group's last row).
+template <class TX, int kMode, bool kPost, int kGate, int kCl>
 __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
     block_norm_backward_kernel(const __grid_constant__ NormBackwardParams p) {
 #if defined(BLACKHOLE_ARCH_SM100)
-  __shared__ __align__(16) float slots[2][2][kCl * 16];
-  const int rank = kCl == 1 ? 0 : static_cast<int>(ptx::cluster_ctarank());
-  const int team = blockIdx.x / kCl;
-  const int T = blockDim.x, tid = threadIdx.x;
-  const int H = p.H;
-  const int c0 = rank * p.slice, c1 = min(H, c0 + p.slice);
+  constexpr bool kLayer = kMode == kLayerNorm, kBias = kMode != kRms;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ RowShared<kCl> sh;
   ptx::pdl_launch_dependents();
-  for (int i = tid; i < 4 * kCl * 16; i += T) (&slots[0][0][0])[i] = 0.f;
-  if constexpr (kCl == 1) __syncthreads();
-  else ptx::cluster_sync();
-  RowSum<kCl, 2> row_sum{slots};
+  RowTeam<kCl> t(sh, ring, p.H, p.slice, p.rows, p.teams, p.stages);
+  RowExchange<kCl> row{sh.slots, sh.counts};
+  const int tid = threadIdx.x, H = p.H;
+  // a stage: h and dh (TX), dy and o (BF16), those that are given
+  const uint32_t xs = uint32_t(p.slice) * sizeof(TX), ys = uint32_t(p.slice) * 2;
+  const uint32_t at_dh = p.dy ? xs : 0, at_dy = at_dh + (p.dh ? xs : 0), at_o = at_dy + (p.dy ? ys : 0);
+  const uint32_t stage_bytes = at_o + (p.o ? ys : 0);
+  const uint32_t xb = uint32_t(t.cols) * sizeof(TX), yb = uint32_t(t.cols) * 2;
+  const uint32_t row_bytes = (p.dy ? xb + yb : 0) + (p.dh ? xb : 0) + (p.o ? yb : 0);
   ptx::pdl_wait_prior_grid();
 
-  int col[2];
-  bool live[2];
+  const uint64_t policy = ptx::l2_policy_evict_first();
+  auto fetch = [&](int64_t r, int stage) {
+    const uint32_t bar = t.bars + 8u * stage, dst = t.ring + stage * stage_bytes;
+    const int64_t at = r * H + t.c0;
+    ptx::mbar_arrive_expect_tx(bar, row_bytes);
+    if (p.dy) {
+      ptx::bulk_load(dst, static_cast<const TX*>(p.h) + at, xb, bar, policy);
+      ptx::bulk_load(dst + at_dy, static_cast<const __nv_bfloat16*>(p.dy) + at, yb, bar, policy);
+    }
+    if (p.dh) ptx::bulk_load(dst + at_dh, static_cast<const TX*>(p.dh) + at, xb, bar, policy);
+    if (p.o) ptx::bulk_load(dst + at_o, static_cast<const __nv_bfloat16*>(p.o) + at, yb, bar, policy);
+  };
+  if (tid == 0)
+    for (int i = 0; i < p.stages && t.row0 + i < t.row1; ++i) fetch(t.row0 + i, i);
+
+  constexpr bool kRegW = !kBias;      // the bias sums leave no registers for the vectors
+  float w[kRegW ? 16 : 1], c[kRegW ? 16 : 1];
+  auto make_c = [&](int64_t g, float (&out)[16]) {
+    vector16(p.gate, g * H, p.gate_bf16, t.col, t.live, 1.f, out);
+    float v[16];
+    if (kPost) vector16(p.post_weight, 0, p.param_bf16, t.col, t.live, 1.f, v);
 #pragma unroll
-  for (int v = 0; v < 2; ++v) {
-    col[v] = c0 + (v * T + tid) * 8;
-    live[v] = col[v] < c1;
-  }
-  const float inv_h = 1.0f / static_cast<float>(H);
-  const int row0 = team * p.rows_per_team, row1 = min(p.rows, row0 + p.rows_per_team);
-  const int64_t vec = int64_t(p.teams) * H;           // floats of one vector's partials
-  float dw[16], db[kLayer ? 16 : 1], dwp[kPost ? 16 : 1], dbp[kPost && kLayer ? 16 : 1],
-      dg[kGate ? 16 : 1];
+    for (int i = 0; i < 16; ++i) out[i] *= kPost ? p.scale * v[i] : p.scale;
+  };
+  if constexpr (kRegW) vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
+  float dw[16], sa[16], db[kBias ? 16 : 1], sb[kBias && kPost ? 16 : 1];
+  float dwp[kGate == 2 && kPost ? 16 : 1], dbp[kGate == 2 && kPost && kBias ? 16 : 1];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    dw[i] = 0.f;
-    if constexpr (kLayer) db[i] = 0.f;
-    if constexpr (kPost) dwp[i] = 0.f;
-    if constexpr (kPost && kLayer) dbp[i] = 0.f;
-    if constexpr (kGate) dg[i] = 0.f;
+    dw[i] = sa[i] = 0.f;
+    if constexpr (kBias) db[i] = 0.f;
+    if constexpr (kBias && kPost) sb[i] = 0.f;
+    if constexpr (kGate == 2 && kPost) dwp[i] = 0.f;
+    if constexpr (kGate == 2 && kPost && kBias) dbp[i] = 0.f;
   }
-  for (int row = row0; row < row1; ++row) {
-    const int64_t at = int64_t(row) * H;
-    const float4 st = reinterpret_cast<const float4*>(p.stats)[row];
-    float d[2][8];                                    // dh', then dp
+  const int64_t vec = int64_t(p.teams) * H;           // floats of one vector's partials
+  auto store16 = [&](float* dst, const float* v) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (t.live[k]) store8(dst + t.col[k], v + 8 * k);
+  };
+  const float inv_h = 1.0f / static_cast<float>(H);
+  int64_t gate_row = -1;
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int64_t r = t.row0; r < t.row1; ++r) {
+    const int64_t at = r * H;
+    const int64_t g = kGate == 2 ? r / p.gate_rows : 0;
+    if constexpr (kRegW) {
+      if (p.o && g != gate_row) {
+        gate_row = g;
+        make_c(g, c);
+      }
+    }
+    const float4 st = reinterpret_cast<const float4*>(p.stats)[r];
+    const uint32_t base = t.ring + stage * stage_bytes;
+    t.wait(stage, phase);
+    float d[16];                                      // dh', then dp
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[v][i] = 0.f;
-      if (live[v] && p.dh) load8(static_cast<const TX*>(p.dh) + at + col[v], d[v]);
+      for (int i = 0; i < 8; ++i) d[8 * v + i] = 0.f;
+      if (t.live[v] && p.dh) shared8<TX>(base + at_dh, t.col[v] - t.c0, d + 8 * v);
     }
     if (p.dy) {
-      float n[2][8], a[2][8], s[2] = {0.f, 0.f};
+      float n[16], a[16], along = 0.f, mean_a = 0.f;
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) n[v][i] = a[v][i] = 0.f;
-        if (!live[v]) continue;
-        load8(static_cast<const TX*>(p.h) + at + col[v], n[v]);
-        load8(static_cast<const __nv_bfloat16*>(p.dy) + at + col[v], a[v]);
-        float w[8];
+        for (int i = 0; i < 8; ++i) n[8 * v + i] = a[8 * v + i] = 0.f;
+        if (!t.live[v]) continue;
+        shared8<TX>(base, t.col[v] - t.c0, n + 8 * v);
+        shared8<__nv_bfloat16>(base + at_dy, t.col[v] - t.c0, a + 8 * v);
+        float wv[8];
+        if constexpr (!kRegW) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = 1.f;
-        if (p.weight) load8_any(p.weight, col[v], p.param_bf16, w);
+          for (int i = 0; i < 8; ++i) wv[i] = 1.f;
+          if (p.weight) load8_any(p.weight, t.col[v], p.param_bf16, wv);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          n[v][i] = (n[v][i] - st.z) * st.w;
-          dw[8 * v + i] = fmaf(a[v][i], n[v][i], dw[8 * v + i]);
-          if constexpr (kLayer) db[8 * v + i] += a[v][i];
-          a[v][i] *= w[i];
-          s[0] = fmaf(a[v][i], n[v][i], s[0]);
-          if constexpr (kLayer) s[1] += a[v][i];
+          const int k = 8 * v + i;
+          n[k] = (n[k] - st.z) * st.w;
+          dw[k] = fmaf(a[k], n[k], dw[k]);
+          if constexpr (kBias) db[k] += a[k];
+          a[k] *= kRegW ? w[kRegW ? k : 0] : wv[i];
+          along = fmaf(a[k], n[k], along);
+          if constexpr (kLayer) mean_a += a[k];
         }
       }
-      row_sum(s);
-      const float along = s[0] * inv_h, mean_a = s[1] * inv_h;
+      row.sum2(along, mean_a, kLayer);
+      along *= inv_h;
+      mean_a *= inv_h;
 #pragma unroll
-      for (int v = 0; v < 2; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (live[v])
-            d[v][i] = fmaf(st.w, a[v][i] - (kLayer ? mean_a : 0.f) - n[v][i] * along, d[v][i]);
+      for (int k = 0; k < 16; ++k)
+        d[k] = fmaf(st.w, fmaf(-n[k], along, kLayer ? a[k] - mean_a : a[k]), d[k]);
     }
 #pragma unroll
     for (int v = 0; v < 2; ++v)
-      if (live[v]) store8(static_cast<TX*>(p.dx) + at + col[v], d[v]);
-    if (!p.o) continue;
-
-    const int group = (kGate && p.gate_rows) ? row / p.gate_rows : 0;
-    float n[2][8], s[2] = {0.f, 0.f};
+      if (t.live[v]) store8(static_cast<TX*>(p.dx) + at + t.col[v], d + 8 * v);
+    float n[16];
+    if (p.o) {
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
+      for (int v = 0; v < 2; ++v) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) n[v][i] = 0.f;
-      if (!live[v]) continue;
-      load8(static_cast<const __nv_bfloat16*>(p.o) + at + col[v], n[v]);
-      float w[8];
-      if constexpr (kPost) {
+        for (int i = 0; i < 8; ++i) n[8 * v + i] = 0.f;
+        if (!t.live[v]) continue;
+        shared8<__nv_bfloat16>(base + at_o, t.col[v] - t.c0, n + 8 * v);
+        float cv[8];
+        if constexpr (!kRegW) {
+          float pw[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) cv[i] = pw[i] = 1.f;
+          if (kGate) load8_any(p.gate, g * H + t.col[v], p.gate_bf16, cv);
+          if (kPost && p.post_weight) load8_any(p.post_weight, t.col[v], p.param_bf16, pw);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) cv[i] *= p.scale * pw[i];
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          n[v][i] = (n[v][i] - st.x) * st.y;
-          w[i] = 1.f;
-        }
-        if (p.post_weight) load8_any(p.post_weight, col[v], p.param_bf16, w);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) d[v][i] *= p.scale;
-      if constexpr (kGate) {
-        float pv[8], g[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pv[i] = kPost ? n[v][i] * w[i] : n[v][i];
-        if (kPost && p.post_bias) {
-          float b[8];
-          load8_any(p.post_bias, col[v], p.param_bf16, b);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pv[i] += b[i];
-        }
-        load8_any(p.gate, int64_t(group) * H + col[v], p.gate_bf16, g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          dg[8 * v + i] = fmaf(d[v][i], pv[i], dg[8 * v + i]);
-          d[v][i] *= g[i];
-        }
-      }
-      if constexpr (kPost) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          dwp[8 * v + i] = fmaf(d[v][i], n[v][i], dwp[8 * v + i]);
-          if constexpr (kLayer) dbp[8 * v + i] += d[v][i];
-          d[v][i] *= w[i];
-          s[0] = fmaf(d[v][i], n[v][i], s[0]);
-          if constexpr (kLayer) s[1] += d[v][i];
+          const int k = 8 * v + i;
+          if constexpr (kPost) n[k] = (n[k] - st.x) * st.y;
+          if (kPost || kGate) sa[k] = fmaf(d[k], n[k], sa[k]);
+          if constexpr (kBias && kPost) sb[k] += d[k];
+          d[k] *= kRegW ? c[kRegW ? k : 0] : cv[i];
         }
       }
     }
-    if constexpr (kPost) {
-      row_sum(s);
-      const float along = s[0] * inv_h, mean_a = s[1] * inv_h;
+    if (kPost) {
+      float along = 0.f, mean_a = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        along = fmaf(t.live[k / 8] ? d[k] : 0.f, n[k], along);
+        if constexpr (kLayer) mean_a += t.live[k / 8] ? d[k] : 0.f;
+      }
+      row.sum2(along, mean_a, kLayer);
+      if (blockDim.x == 32) __syncwarp();
+      along *= inv_h;
+      mean_a *= inv_h;
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        d[k] = st.y * fmaf(-n[k], along, kLayer ? d[k] - mean_a : d[k]);
+    } else {
+      t.release_barrier();                            // every thread has read the stage
+    }
+    if (tid == 0 && r + p.stages < t.row1) fetch(r + p.stages, stage);
+    if (p.o)
 #pragma unroll
       for (int v = 0; v < 2; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          d[v][i] = st.y * (d[v][i] - (kLayer ? mean_a : 0.f) - n[v][i] * along);
-    }
-#pragma unroll
-    for (int v = 0; v < 2; ++v)
-      if (live[v]) store8(static_cast<__nv_bfloat16*>(p.d_o) + at + col[v], d[v]);
+        if (t.live[v]) store8(static_cast<__nv_bfloat16*>(p.d_o) + at + t.col[v], d + 8 * v);
 
-    if constexpr (kGate) {
-      // last row of this gate row's group in this team: the sum is whole (stored), or an edge
-      // piece for the second kernel: slot 0 if the group began in an earlier team, else slot 1
-      const bool last = row + 1 == row1 || (p.gate_rows && (row + 1) % p.gate_rows == 0);
-      if (last) {
-        const int64_t g0 = int64_t(group) * p.gate_rows;
-        const int64_t g1 = p.gate_rows ? min(int64_t(p.rows), g0 + p.gate_rows) : p.rows;
+    if constexpr (kGate == 2) {
+      const int64_t g0 = g * p.gate_rows, g1 = min(int64_t(p.rows), g0 + p.gate_rows);
+      if (r + 1 == t.row1 || r + 1 == g1) {
+        // close the group's sums in this team: the whole group's (stored), or an edge piece for
+        // the second kernel: slot 0 if the group began in an earlier team, else slot 1
         if (p.dgate) {
-          float* dst = g0 >= row0 && g1 <= row1 ? p.dgate + int64_t(group) * H
-                                                : p.ws + (g0 < row0 ? 4 : 5) * vec + int64_t(team) * H;
+          float v[16], u[16];
+          vector16(kPost ? p.post_weight : nullptr, 0, p.param_bf16, t.col, t.live, 1.f, v);
+          vector16(kPost && kBias ? p.post_bias : nullptr, 0, p.param_bf16, t.col, t.live, 0.f, u);
 #pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            float t[8];
+          for (int k = 0; k < 16; ++k) {
+            v[k] *= p.scale * sa[k];
+            if constexpr (kBias && kPost) v[k] = fmaf(p.scale * u[k], sb[k], v[k]);
+          }
+          store16(g0 >= t.row0 && g1 <= t.row1 ? p.dgate + g * H
+                                               : p.ws + (g0 < t.row0 ? 4 : 5) * vec + int64_t(t.team) * H, v);
+        }
+        if constexpr (kPost) {
+          float v[16];
+          vector16(p.gate, g * H, p.gate_bf16, t.col, t.live, 1.f, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = dg[8 * v + i];
-            if (live[v]) store8(dst + col[v], t);
+          for (int k = 0; k < 16; ++k) {
+            dwp[k] = fmaf(p.scale * v[k], sa[k], dwp[k]);
+            if constexpr (kBias) dbp[k] = fmaf(p.scale * v[k], sb[k], dbp[k]);
           }
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) dg[i] = 0.f;
+        for (int k = 0; k < 16; ++k) {
+          sa[k] = 0.f;
+          if constexpr (kBias && kPost) sb[k] = 0.f;
+        }
+      }
+    }
+    if (++stage == p.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  float* const mine = p.ws + int64_t(t.team) * H;
+  if (p.dweight) store16(mine, dw);
+  if constexpr (kBias)
+    if (p.dbias) store16(mine + vec, db);
+  if constexpr (kGate == 2 && kPost) {
+    if (p.dpost_weight) store16(mine + 2 * vec, dwp);
+    if constexpr (kBias)
+      if (p.dpost_bias) store16(mine + 3 * vec, dbp);
+  } else if constexpr (kPost || kGate == 1) {
+    float gv[16];
+    vector16(kGate ? p.gate : nullptr, 0, p.gate_bf16, t.col, t.live, 1.f, gv);
+    if (kGate && p.dgate) {          // the only group; a team's piece of it (slot 1 of the first)
+      float v[16], u[16];
+      vector16(kPost ? p.post_weight : nullptr, 0, p.param_bf16, t.col, t.live, 1.f, v);
+      vector16(kPost && kBias ? p.post_bias : nullptr, 0, p.param_bf16, t.col, t.live, 0.f, u);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        v[k] *= p.scale * sa[k];
+        if constexpr (kBias && kPost) v[k] = fmaf(p.scale * u[k], sb[k], v[k]);
+      }
+      store16(p.teams == 1 ? p.dgate : mine + (t.team ? 4 : 5) * vec, v);
+    }
+    if constexpr (kPost) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) sa[k] *= p.scale * gv[k];
+      if (p.dpost_weight) store16(mine + 2 * vec, sa);
+      if constexpr (kBias) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sb[k] *= p.scale * gv[k];
+        if (p.dpost_bias) store16(mine + 3 * vec, sb);
       }
     }
   }
-  auto park = [&](const float* out, int which, const float* acc) {
-    if (!out) return;
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      float t[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = acc[8 * v + i];
-      if (live[v]) store8(p.ws + which * vec + int64_t(team) * H + col[v], t);
-    }
-  };
-  park(p.dweight, 0, dw);
-  if constexpr (kLayer) park(p.dbias, 1, db);
-  if constexpr (kPost) park(p.dpost_weight, 2, dwp);
-  if constexpr (kPost && kLayer) park(p.dpost_bias, 3, dbp);
   if constexpr (kCl > 1) ptx::cluster_sync();
 #endif
 }
 
-// Adds the teams' partials: y = 0..3 the four parameter vectors, y = 3 + c (c = 1..teams-1) the
-// gate group that crosses into team c, if c is the first team it crosses into.
+// Adds the teams' partials: y = 0..3 the four parameter vectors, then the gate groups that cross
+// from one team into another.  by_group (no more groups than teams): y - 4 is the group; else
+// y - 3 is a team, and the group is the one that crosses into it if it is the first it crosses into.
 static __global__ void __launch_bounds__(1024)
     block_norm_sums_kernel(const __grid_constant__ NormBackwardParams p) {
   __shared__ float smem[32 * 33];
@@ -666,29 +909,57 @@ static __global__ void __launch_bounds__(1024)
     detail::column_sum_cta(nullptr, p.ws + blockIdx.y * vec, p.teams, p.H, dst, p.H, blockIdx.x, smem);
     return;
   }
-  const int c = static_cast<int>(blockIdx.y) - 3;
-  const int64_t R = p.rows_per_team, at = c * R;      // first row of team c
   const int64_t gr = p.gate_rows ? p.gate_rows : p.rows;
-  const int64_t g = at / gr, g0 = g * gr, g1 = min(int64_t(p.rows), g0 + gr);
-  if (g0 >= at || g0 / R != c - 1) return;            // starts here, or crossed in earlier
-  const int last = static_cast<int>((g1 - 1) / R);
-  detail::column_sum_cta(p.ws + 5 * vec + int64_t(c - 1) * p.H, p.ws + 4 * vec + int64_t(c) * p.H,
-                         last - c + 1, p.H, p.dgate + g * p.H, p.H, blockIdx.x, smem);
+  int64_t g;
+  if (p.groups <= p.teams) {
+    g = blockIdx.y - 4;
+  } else {
+    const int64_t into = int64_t(blockIdx.y) - 3, at = row_begin(into, p.rows, p.teams);
+    g = at / gr;
+    if (g * gr >= at || team_of(g * gr, p.rows, p.teams) != into - 1) return;
+  }
+  const int64_t first = team_of(g * gr, p.rows, p.teams);
+  const int64_t last = team_of(min(int64_t(p.rows), (g + 1) * gr) - 1, p.rows, p.teams);
+  if (first == last) return;                          // stored whole by its team
+  detail::column_sum_cta(p.ws + 5 * vec + first * p.H, p.ws + 4 * vec + (first + 1) * p.H, last - first,
+                         p.H, p.dgate + g * p.H, p.H, blockIdx.x, smem);
 }
 
-template <class TX, bool kLayer, bool kPost>
-inline cudaError_t launch_block_norm(const NormParams& p, const Geometry& g, cudaStream_t s) {
-  auto* kernel = g.cluster == 1 ? block_norm_kernel<TX, kLayer, kPost, 1>
-                                : block_norm_kernel<TX, kLayer, kPost, 2>;
-  return detail::launch_pdl(kernel, dim3(p.teams * g.cluster), dim3(g.threads), 0, s, p);
+template <class P>
+inline cudaError_t launch_rows(void (*kernel)(P), P& p, const Geometry& g, int stage_bytes, cudaStream_t s) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  e = detail::set_smem_once(kernel, kRingBytesPerSm, dev);
+  if (e != cudaSuccess) return e;
+  p.slice = g.slice;
+  p.teams = row_teams(p.rows, g);
+  p.stages = ring_stages(g, stage_bytes, (p.rows + p.teams - 1) / p.teams);
+  return detail::launch_pdl(kernel, dim3(p.teams * g.cluster), dim3(g.threads),
+                            static_cast<size_t>(p.stages) * stage_bytes, s, p);
 }
 
-template <class TX, bool kLayer, bool kPost, bool kGate>
-inline cudaError_t launch_block_norm_backward(const NormBackwardParams& p, const Geometry& g,
-                                              cudaStream_t s) {
-  auto* kernel = g.cluster == 1 ? block_norm_backward_kernel<TX, kLayer, kPost, kGate, 1>
-                                : block_norm_backward_kernel<TX, kLayer, kPost, kGate, 2>;
-  return detail::launch_pdl(kernel, dim3(p.teams * g.cluster), dim3(g.threads), 0, s, p);
+template <class TX, int kMode>
+inline cudaError_t launch_block_norm(NormParams& p, bool post, cudaStream_t s) {
+  const Geometry g = geometry(p.H);
+  auto* kernel = g.cluster == 1 ? (post ? block_norm_kernel<TX, kMode, true, 1> : block_norm_kernel<TX, kMode, false, 1>)
+                                : (post ? block_norm_kernel<TX, kMode, true, 2> : block_norm_kernel<TX, kMode, false, 2>);
+  return launch_rows(kernel, p, g, g.slice * int(sizeof(TX) + (p.o ? 2 : 0)), s);
+}
+
+template <class TX, int kMode, bool kPost, int kGate>
+inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, cudaStream_t s) {
+  const Geometry g = geometry(p.H);
+  auto* kernel = g.cluster == 1 ? block_norm_backward_kernel<TX, kMode, kPost, kGate, 1>
+                                : block_norm_backward_kernel<TX, kMode, kPost, kGate, 2>;
+  const int per = (p.dy ? int(sizeof(TX)) + 2 : 0) + (p.dh ? int(sizeof(TX)) : 0) + (p.o ? 2 : 0);
+  return launch_rows(kernel, p, g, g.slice * per, s);
+}
+template <class TX, int kMode, bool kPost>
+inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, int gate, cudaStream_t s) {
+  return gate == 0   ? launch_block_norm_backward<TX, kMode, kPost, 0>(p, s)
+         : gate == 1 ? launch_block_norm_backward<TX, kMode, kPost, 1>(p, s)
+                     : launch_block_norm_backward<TX, kMode, kPost, 2>(p, s);
 }
 
 }  // namespace norm_detail
@@ -697,26 +968,22 @@ inline cudaError_t block_norm(const blackhole_sm100_block_norm_args& a, cudaStre
   using namespace norm_detail;
   cudaError_t e = block_norm_check(a);
   if (e != cudaSuccess) return e;
-  const Geometry g = geometry(a.H);
   NormParams p;
   p.x = a.x; p.o = a.o; p.gate = a.gate; p.weight = a.weight; p.bias = a.bias;
   p.post_weight = a.post_weight; p.post_bias = a.post_bias;
   p.h = a.h; p.out = a.out; p.sf = static_cast<uint8_t*>(a.sf); p.stats = a.stats;
-  p.rows = a.rows; p.H = a.H; p.slice = g.slice;
-  p.teams = std::min(a.rows, 148 * 16);
+  p.rows = a.rows; p.H = a.H;
   p.gate_rows = a.gate ? a.gate_rows : 0;
   p.param_bf16 = a.param_is_bf16; p.gate_bf16 = a.gate_is_bf16; p.out_format = a.out_format;
   p.scale = a.scale; p.eps = a.eps; p.global_scale = a.global_scale;
-  const bool layer = a.kind == 1, post = a.post_norm != 0;
-  if (a.x_is_bf16) {
-    using T = __nv_bfloat16;
-    e = layer ? (post ? launch_block_norm<T, true, true>(p, g, stream) : launch_block_norm<T, true, false>(p, g, stream))
-              : (post ? launch_block_norm<T, false, true>(p, g, stream) : launch_block_norm<T, false, false>(p, g, stream));
-  } else {
-    using T = float;
-    e = layer ? (post ? launch_block_norm<T, true, true>(p, g, stream) : launch_block_norm<T, true, false>(p, g, stream))
-              : (post ? launch_block_norm<T, false, true>(p, g, stream) : launch_block_norm<T, false, false>(p, g, stream));
-  }
+  const bool post = a.post_norm != 0;
+  auto run = [&](auto tx) {
+    using T = decltype(tx);
+    return a.kind == 1              ? launch_block_norm<T, kLayerNorm>(p, post, stream)
+           : a.bias || a.post_bias  ? launch_block_norm<T, kRmsBias>(p, post, stream)
+                                    : launch_block_norm<T, kRms>(p, post, stream);
+  };
+  e = a.x_is_bf16 ? run(__nv_bfloat16{}) : run(float{});
   if (e != cudaSuccess) return e;
   return cudaGetLastError();
 }
@@ -726,8 +993,6 @@ inline cudaError_t block_norm_backward(const blackhole_sm100_block_norm_backward
   using namespace norm_detail;
   cudaError_t e = block_norm_backward_check(a);
   if (e != cudaSuccess) return e;
-  const Geometry g = geometry(a.H);
-  const Teams t = backward_teams(a.rows, a.H);
   NormBackwardParams p;
   p.h = a.h; p.dy = a.dy; p.dh = a.dh; p.o = a.o; p.gate = a.gate; p.weight = a.weight;
   p.post_weight = a.post_weight; p.post_bias = a.post_bias; p.stats = a.stats;
@@ -735,29 +1000,30 @@ inline cudaError_t block_norm_backward(const blackhole_sm100_block_norm_backward
   p.dweight = a.dweight; p.dbias = a.dbias; p.dpost_weight = a.dpost_weight;
   p.dpost_bias = a.dpost_bias; p.dgate = a.dgate;
   p.ws = static_cast<float*>(a.workspace);
-  p.rows = a.rows; p.H = a.H; p.slice = g.slice; p.teams = t.teams; p.rows_per_team = t.rows_per_team;
+  p.rows = a.rows; p.H = a.H;
   p.gate_rows = a.gate ? a.gate_rows : 0;
+  p.groups = !a.gate || a.gate_rows == 0 ? 1 : static_cast<int>((int64_t(a.rows) + a.gate_rows - 1) / a.gate_rows);
   p.param_bf16 = a.param_is_bf16; p.gate_bf16 = a.gate_is_bf16;
   p.scale = a.scale;
+  // one group closes its sums once, at a team's end
+  const int gate = !a.gate ? 0 : p.groups == 1 ? 1 : 2;
+  const bool bias = a.dbias || a.dpost_bias || (a.post_bias && a.dgate);
   auto run = [&](auto tx) {
     using T = decltype(tx);
-    const int sel = (a.kind == 1 ? 4 : 0) + (a.post_norm ? 2 : 0) + (a.gate ? 1 : 0);
-    switch (sel) {
-      case 0: return launch_block_norm_backward<T, false, false, false>(p, g, stream);
-      case 1: return launch_block_norm_backward<T, false, false, true>(p, g, stream);
-      case 2: return launch_block_norm_backward<T, false, true, false>(p, g, stream);
-      case 3: return launch_block_norm_backward<T, false, true, true>(p, g, stream);
-      case 4: return launch_block_norm_backward<T, true, false, false>(p, g, stream);
-      case 5: return launch_block_norm_backward<T, true, false, true>(p, g, stream);
-      case 6: return launch_block_norm_backward<T, true, true, false>(p, g, stream);
-      default: return launch_block_norm_backward<T, true, true, true>(p, g, stream);
-    }
+    if (a.kind == 1)
+      return a.post_norm ? launch_block_norm_backward<T, kLayerNorm, true>(p, gate, stream)
+                         : launch_block_norm_backward<T, kLayerNorm, false>(p, gate, stream);
+    if (bias)
+      return a.post_norm ? launch_block_norm_backward<T, kRmsBias, true>(p, gate, stream)
+                         : launch_block_norm_backward<T, kRmsBias, false>(p, gate, stream);
+    return a.post_norm ? launch_block_norm_backward<T, kRms, true>(p, gate, stream)
+                       : launch_block_norm_backward<T, kRms, false>(p, gate, stream);
   };
   e = a.x_is_bf16 ? run(__nv_bfloat16{}) : run(float{});
   if (e != cudaSuccess) return e;
-  const bool edges = a.dgate && p.gate_rows != 1 && t.teams > 1;
+  const int edges = a.dgate && a.gate_rows != 1 && p.teams > 1 ? std::min(p.groups, p.teams - 1 + (p.groups <= p.teams)) : 0;
   if (a.dweight || a.dbias || a.dpost_weight || a.dpost_bias || edges) {
-    const dim3 grid((a.H + 31) / 32, 4 + (edges ? t.teams - 1 : 0));
+    const dim3 grid((a.H + 31) / 32, 4 + edges);
     e = detail::launch_pdl(block_norm_sums_kernel, grid, dim3(1024), 0, stream, p);
     if (e != cudaSuccess) return e;
   }
