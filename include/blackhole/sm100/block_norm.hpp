@@ -163,29 +163,72 @@ inline cudaError_t block_norm_backward_check(const blackhole_sm100_block_norm_ba
 
 namespace norm_detail {
 
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 q = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+// 8 values of a vector of parameters or gates, BF16 or FP32 (uniform over the launch).
+__device__ __forceinline__ void load8_any(const void* p, int64_t at, int is_bf16, float (&v)[8]) {
+  if (is_bf16) {
+    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + at);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  } else {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    const float4 a = q[0], b = q[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
 }
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-// A vector of parameters or gates, BF16 or FP32 (uniform over the launch).
-__device__ __forceinline__ void load8_any(const void* p, int64_t at, int is_bf16, float (&v)[8]) {
-  if (is_bf16) load8(static_cast<const __nv_bfloat16*>(p) + at, v);
-  else load8(static_cast<const float*>(p) + at, v);
-}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
+}
+
+// Pairs of FP32 values, as sm_100's packed FP32 instructions take them: half the issue slots of
+// one value at a time (these kernels were bound by instruction issue before).
+__device__ __forceinline__ uint64_t pair_bits(float2 v) { return (uint64_t(__float_as_uint(v.y)) << 32) | __float_as_uint(v.x); }
+__device__ __forceinline__ float2 pair_of(uint64_t b) {
+  return make_float2(__uint_as_float(uint32_t(b)), __uint_as_float(uint32_t(b >> 32)));
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+  return pair_of(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return pair_of(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return pair_of(d);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// A thread's 16 columns of a row, as 8 pairs: pairs 0-3 its first 8-column vector, 4-7 its second.
+using Row16 = float2[8];
+
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+// 8 values at element `at` of a row in shared memory.
+template <class T>
+__device__ __forceinline__ void shared8(uint32_t row, int at, float2* v) {
+  if constexpr (sizeof(T) == 2) {
+    const uint4 q = ptx::ld_shared_v4(row + 2 * at);
+    v[0] = unpack2(q.x); v[1] = unpack2(q.y); v[2] = unpack2(q.z); v[3] = unpack2(q.w);
+  } else {
+    const uint4 a = ptx::ld_shared_v4(row + 4 * at), b = ptx::ld_shared_v4(row + 4 * at + 16);
+    v[0] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y));
+    v[1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
+    v[2] = make_float2(__uint_as_float(b.x), __uint_as_float(b.y));
+    v[3] = make_float2(__uint_as_float(b.z), __uint_as_float(b.w));
+  }
 }
 
 // Exchange of one pair of values per warp across a row's CTA or cluster.  Two slot sets in turn: a
@@ -220,65 +263,91 @@ struct RowExchange {
     }
   }
   __device__ __forceinline__ float total(int k) const {
-    float s = 0.f;
     const float4* q = reinterpret_cast<const float4*>(slots[set][k]);
+    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < kWarps / 4; ++i) {
       const float4 t = q[i];
-      s += (t.x + t.y) + (t.z + t.w);
+      s = add2(s, add2(make_float2(t.x, t.y), make_float2(t.z, t.w)));
     }
+    return s.x + s.y;
+  }
+  // Sums over the row, the same in every thread, added in a fixed order.  A barrier of the CTA or
+  // cluster, unless the CTA is one warp.
+  __device__ __forceinline__ float sum(float2 v) {
+    const float a = warp_sum(v.x + v.y);
+    if (kCl == 1 && blockDim.x == 32) return a;
+    put(a, 0.f);
+    const float s = total(0);
+    set ^= 1;
     return s;
   }
-  // Sums of a and b over the row, the same in every thread, added in a fixed order.  A barrier
-  // of the CTA or cluster, unless the CTA is one warp.
-  __device__ __forceinline__ void sum2(float& a, float& b, bool with_b) {
-    a = warp_sum(a);
-    if (with_b) b = warp_sum(b);
+  __device__ __forceinline__ void sum2(float2 va, float2 vb, float& a, float& b) {
+    a = warp_sum(va.x + va.y);
+    b = warp_sum(vb.x + vb.y);
     if (kCl == 1 && blockDim.x == 32) return;
     put(a, b);
     a = total(0);
-    if (with_b) b = total(1);
+    b = total(1);
     set ^= 1;
   }
-  // Mean and sum of squares about it of the row's values (16 per thread): each warp's own mean
+  // Mean and sum of squares about it of the row's values (0 past its end): each warp's own mean
   // and squares about that first, then merged, so nothing cancels however far the mean is from
   // zero, and one barrier is enough.
-  __device__ __forceinline__ void mean_squares(const float (&v)[16], const bool (&live)[2], float inv_h,
+  __device__ __forceinline__ void mean_squares(const Row16& v, const bool (&live)[2], float inv_h,
                                                float& mean, float& squares) {
     const int me = (kCl == 1 ? 0 : int(ptx::cluster_ctarank())) * 16 + (threadIdx.x >> 5);
-    float s = 0.f;
+    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += v[i];
+    for (int i = 0; i < 8; ++i) s = add2(s, v[i]);
     const float n = counts[me];
-    const float mw = n > 0.f ? warp_sum(s) / n : 0.f;
-    float m2 = 0.f;
+    const float mw = n > 0.f ? warp_sum(s.x + s.y) / n : 0.f;
+    float2 q2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float d = v[i] - mw;
-      m2 += live[i / 8] ? d * d : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      const float2 d = add2(v[i], both(-mw));
+      q2[i / 4] = fma2(d, d, q2[i / 4]);
     }
-    m2 = warp_sum(m2);
+    const float m2 = warp_sum((live[0] ? q2[0].x + q2[0].y : 0.f) + (live[1] ? q2[1].x + q2[1].y : 0.f));
     if (kCl == 1 && blockDim.x == 32) {
       mean = mw;
       squares = m2;
       return;
     }
     put(mw, m2);
-    float total_mean = 0.f;
+    const float4 *mq = reinterpret_cast<const float4*>(slots[set][0]), *cq = reinterpret_cast<const float4*>(counts);
+    float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) total_mean = fmaf(counts[i], slots[set][0][i], total_mean);
-    total_mean *= inv_h;
-    float q = total(1);
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const float d = slots[set][0][i] - total_mean;
-      q = fmaf(counts[i] * d, d, q);
+    for (int i = 0; i < kWarps / 4; ++i) {
+      const float4 m = mq[i], c = cq[i];
+      t = fma2(make_float2(m.x, m.y), make_float2(c.x, c.y), t);
+      t = fma2(make_float2(m.z, m.w), make_float2(c.z, c.w), t);
     }
-    mean = total_mean;
-    squares = q;
+    mean = (t.x + t.y) * inv_h;
+    float2 q = make_float2(total(1), 0.f);
+#pragma unroll
+    for (int i = 0; i < kWarps / 4; ++i) {
+      const float4 m = mq[i], c = cq[i];
+      const float2 d0 = add2(make_float2(m.x, m.y), both(-mean)), d1 = add2(make_float2(m.z, m.w), both(-mean));
+      q = fma2(mul2(d0, make_float2(c.x, c.y)), d0, q);
+      q = fma2(mul2(d1, make_float2(c.z, c.w)), d1, q);
+    }
+    squares = q.x + q.y;
     set ^= 1;
   }
 };
+
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float2* v) {
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(detail::pack_bf16x2(v[0].x, v[0].y), detail::pack_bf16x2(v[1].x, v[1].y),
+                   detail::pack_bf16x2(v[2].x, v[2].y), detail::pack_bf16x2(v[3].x, v[3].y));
+  } else {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+  }
+}
 
 // Shared memory of a CTA: the ring's stages first (dynamic), then this.
 template <int kCl>
@@ -294,26 +363,27 @@ template <int kCl>
 struct RowTeam {
   int rank, team, col[2];
   bool live[2];
-  int64_t row0, row1;
-  int c0, cols;                  // the CTA's columns of a row
+  int row0, row1;
+  int c0, cols, width;           // the CTA's columns of a row; a stage row's, 16 per thread
   uint32_t ring, bars;
   volatile int* abort_flag;
 
   __device__ __forceinline__ RowTeam(RowShared<kCl>& sh, uint8_t* ring_ptr, int H, int slice, int rows,
-                                     int teams, int stages) {
+                                     int teams, int stages, uint32_t ring_bytes) {
     rank = kCl == 1 ? 0 : static_cast<int>(ptx::cluster_ctarank());
     team = blockIdx.x / kCl;
     const int T = blockDim.x, tid = threadIdx.x;
     c0 = rank * slice;
     const int c1 = min(H, c0 + slice);
     cols = c1 - c0;
+    width = 16 * T;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
       col[v] = c0 + (v * T + tid) * 8;
       live[v] = col[v] < c1;
     }
-    row0 = row_begin(team, rows, teams);
-    row1 = row_begin(team + 1, rows, teams);
+    row0 = static_cast<int>(row_begin(team, rows, teams));
+    row1 = static_cast<int>(row_begin(team + 1, rows, teams));
     ring = ptx::smem_u32(ring_ptr);
     bars = ptx::smem_u32(sh.bars);
     abort_flag = &sh.abort_flag;
@@ -328,6 +398,9 @@ struct RowTeam {
       }
       sh.counts[i] = static_cast<float>(n);
     }
+    // columns past the row's end read as 0: no copy writes there
+    if (cols != width)
+      for (uint32_t i = 16 * tid; i < ring_bytes; i += 16 * T) ptx::st_shared_v4(ring + i, 0, 0, 0, 0);
     if (tid == 0) {
       for (int s = 0; s < stages; ++s) ptx::mbar_init(bars + 8u * s, 1);
       sh.abort_flag = 0;
@@ -342,58 +415,52 @@ struct RowTeam {
   __device__ __forceinline__ void wait(int stage, uint32_t phase) {
     (void)ptx::wait_bounded(bars + 8u * stage, phase, abort_flag, &detail::g_status, kStatusLoadTimeout);
   }
+  // This thread's 16 values of a row in shared memory, 0 past its end.
+  template <class T>
+  __device__ __forceinline__ void read16(uint32_t row, Row16& v) const {
+    shared8<T>(row, threadIdx.x * 8, v);
+    shared8<T>(row, (blockDim.x + threadIdx.x) * 8, v + 4);
+  }
+  template <class T>
+  __device__ __forceinline__ void write16(T* row, const Row16& v) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (live[k]) store8(row + col[k], v + 4 * k);
+  }
   // Every thread of the CTA has read the stage.
   __device__ __forceinline__ void release_barrier() const { __syncthreads(); }
 };
 
-__device__ __forceinline__ uint4 lds16(uint32_t a) { return ptx::ld_shared_v4(a); }
-__device__ __forceinline__ void unpack8(const uint4& q, float* v) {
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
-// 8 values at element `at` of a row in shared memory.
-template <class T>
-__device__ __forceinline__ void shared8(uint32_t row, int at, float* v) {
-  if constexpr (sizeof(T) == 2) {
-    unpack8(lds16(row + 2 * at), v);
-  } else {
-    const uint4 a = lds16(row + 4 * at), b = lds16(row + 4 * at + 16);
-    v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
-    v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
-  }
-}
-template <class T>
-__device__ __forceinline__ void store8(T* p, const float* v) {
-  if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<uint4*>(p) =
-        make_uint4(detail::pack_bf16x2(v[0], v[1]), detail::pack_bf16x2(v[2], v[3]),
-                   detail::pack_bf16x2(v[4], v[5]), detail::pack_bf16x2(v[6], v[7]));
-  } else {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  }
-}
-// This thread's 16 values of a parameter vector (BF16 or FP32), `none` where it is absent.
+// This thread's 16 values of a parameter vector (BF16 or FP32): `none` where it is absent, 0 past
+// the row's end.
 __device__ __forceinline__ void vector16(const void* p, int64_t at, int is_bf16, const int (&col)[2],
-                                         const bool (&live)[2], float none, float (&out)[16]) {
+                                         const bool (&live)[2], float none, Row16& out) {
 #pragma unroll
   for (int v = 0; v < 2; ++v) {
     float t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = none;
+    for (int i = 0; i < 8; ++i) t[i] = live[v] ? none : 0.f;
     if (p && live[v]) load8_any(p, at + col[v], is_bf16, t);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[8 * v + i] = t[i];
+    for (int i = 0; i < 4; ++i) out[4 * v + i] = make_float2(t[2 * i], t[2 * i + 1]);
   }
 }
 
 // What a kernel is built for: RMS norms, RMS norms with a bias (or its gradient) somewhere, layer
 // norms.
 enum NormMode : int { kRms = 0, kRmsBias = 1, kLayerNorm = 2 };
+
+// E2M1 codes of eight values (round to nearest even, finite values past 6 saturate; NaN as 6, the
+// conversion of nvfp4_quant.hpp's e2m1_rne), the first in the lowest nibble.
+__device__ __forceinline__ uint32_t e2m1x8(const float2 (&v)[4]) {
+  return quant_detail::e2m1x4_cvt(v[0].x, v[0].y, v[1].x, v[1].y) |
+         (quant_detail::e2m1x4_cvt(v[2].x, v[2].y, v[3].x, v[3].y) << 16);
+}
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float d;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 struct NormParams {
   const void *x, *o, *gate, *weight, *bias, *post_weight, *post_bias;
@@ -405,51 +472,78 @@ struct NormParams {
   float scale, eps, global_scale;
 };
 
-// Quantises 8 consecutive columns of this thread's row; neighbouring lanes hold the other
-// columns of the 16- or 32-column block.  Every lane of the warp calls it (`live` false: past
-// the row's end, all zero).  Recipes and roundings are those of nvfp4_quant.hpp.
-template <class Store32, class Store64>
-__device__ __forceinline__ uint32_t quantize8(const float* y, bool live, int fmt, float g,
-                                              Store32 store32, Store64 store64) {
-  float m = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(y[i]));
+// Quantises 8 consecutive columns of this thread's row into `out` (the row's codes); neighbouring
+// lanes hold the other columns of the 16- or 32-column block.  Every lane of the warp calls it
+// (`live` false: past the row's end, all zero).  Recipes and roundings are those of
+// nvfp4_quant.hpp.  Returns the block's scale factor code.
+template <int kFmt>
+__device__ __forceinline__ uint32_t quantize8(const float2* y, bool live, float g, float c, uint8_t* out, int col) {
+  float m = max_abs3(max_abs3(max_abs3(y[0].x, y[0].y, y[1].x), y[1].y, y[2].x), y[2].y, y[3].x);
+  m = max_abs3(m, y[3].y, 0.f);
   m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-  uint32_t code = 0;
-  if (fmt == kOutNvfp4) {
-    uint32_t q = 0;
+  float2 v[4];
+  if constexpr (kFmt == kOutNvfp4) {
+    uint32_t q = 0, code = 0;
     if (live && m > 0.f) {
-      code = quant_detail::ue4m3_cvt((m / 6.0f) / g);
+      // as in quantize_kernel: estimates, and exact quotients only next to a rounding threshold
+      const float ys = m * c;
+      code = quant_detail::ue4m3_cvt(quant_detail::near_ue4m3_threshold(ys) ? (m / 6.0f) / g : ys);
       const float s = quant_detail::ue4m3_value(code);
       if (s != 0.f) {
         const float scale = s * g;
-        q = quant_detail::e2m1x4_cvt(y[0] / scale, y[1] / scale, y[2] / scale, y[3] / scale) |
-            (quant_detail::e2m1x4_cvt(y[4] / scale, y[5] / scale, y[6] / scale, y[7] / scale) << 16);
+        const float rs = quant_detail::rcp_approx(scale);
+        bool near = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = mul2(y[i], both(rs));
+          near |= quant_detail::near_e2m1_threshold(v[i].x) || quant_detail::near_e2m1_threshold(v[i].y);
+        }
+        if (near) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = make_float2(y[i].x / scale, y[i].y / scale);
+        }
+        q = e2m1x8(v);
       }
     }
-    store32(q);
+    if (live) *reinterpret_cast<uint32_t*>(out + col / 2) = q;
     return code;
-  }
-  m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-  const int ebits = static_cast<int>((__float_as_uint(m) >> 23) & 0xFFu);
-  int e = ebits == 0 ? -127 : ebits - (fmt == kOutMxfp8 ? 135 : 129);
-  e = max(-127, min(127, e));
-  code = live ? static_cast<uint32_t>(e + 127) : 0u;
-  const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-  if (fmt == kOutMxfp4) {
-    uint32_t q = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q |= quant_detail::e2m1_rne(y[i] * inv) << (4 * i);
-    store32(q);
   } else {
-    uint32_t w[2];
+    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+    const int ebits = static_cast<int>(__float_as_uint(m) >> 23);
+    const int e = ebits == 0 ? -127 : max(-127, ebits - (kFmt == kOutMxfp8 ? 135 : 129));   // <= 126
+    const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      w[i] = quant_detail::e4m3x2_satfinite(y[4 * i] * inv, y[4 * i + 1] * inv) |
-             (quant_detail::e4m3x2_satfinite(y[4 * i + 2] * inv, y[4 * i + 3] * inv) << 16);
-    store64(make_uint2(w[0], w[1]));
+    for (int i = 0; i < 4; ++i) v[i] = mul2(y[i], both(inv));
+    if constexpr (kFmt == kOutMxfp4) {
+      const uint32_t q = e2m1x8(v);
+      if (live) *reinterpret_cast<uint32_t*>(out + col / 2) = q;
+    } else {
+      const uint32_t lo = quant_detail::e4m3x2_satfinite(v[0].x, v[0].y) | (quant_detail::e4m3x2_satfinite(v[1].x, v[1].y) << 16);
+      const uint32_t hi = quant_detail::e4m3x2_satfinite(v[2].x, v[2].y) | (quant_detail::e4m3x2_satfinite(v[3].x, v[3].y) << 16);
+      if (live) *reinterpret_cast<uint2*>(out + col) = make_uint2(lo, hi);
+    }
+    return live ? static_cast<uint32_t>(e + 127) : 0u;
   }
-  return code;
+}
+
+// A row's 16 columns of this thread, quantised, and the words of their scale factors: four groups'
+// codes, on 8 (NVFP4) or 16 neighbouring lanes, make one word of the row.
+template <int kFmt, class Team>
+__device__ __forceinline__ void quantize_row(const Row16& y, const Team& t, float g, float c, void* out,
+                                             uint8_t* sf, int64_t r, int H) {
+  constexpr int kVec = kFmt == kOutNvfp4 ? 16 : 32, kPer = kVec / 8, kLanes = 4 * kPer;
+  const int lane = threadIdx.x & 31, ri = static_cast<int>(r);
+  uint8_t* const row = static_cast<uint8_t*>(out) + (kFmt == kOutMxfp8 ? r * H : r * H / 2);
+  uint8_t* const sf_row = sf + int64_t(ri >> 7) * ((H / kVec + 3) / 4) * 512 + (ri & 31) * 16 + ((ri >> 5) & 3) * 4;
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    const uint32_t code = quantize8<kFmt>(y + 4 * v, t.live[v], g, c, row, t.col[v]);
+    uint32_t word = (lane % kPer) == 0 ? code << (8 * ((lane / kPer) & 3)) : 0u;
+#pragma unroll
+    for (int k = kPer; k < kLanes; k <<= 1) word |= __shfl_xor_sync(0xFFFFFFFFu, word, k);
+    if ((lane % kLanes) == 0 && t.live[v])
+      *reinterpret_cast<uint32_t*>(sf_row + (t.col[v] / (4 * kVec)) * 512) = word;
+  }
 }
 
 // Forward.  kPost and p.o select what a row's p is made of; the gate row, the scale and the post
@@ -463,153 +557,115 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ RowShared<kCl> sh;
   ptx::pdl_launch_dependents();
-  RowTeam<kCl> t(sh, ring, p.H, p.slice, p.rows, p.teams, p.stages);
+  const uint32_t x_row = uint32_t(blockDim.x) * 16 * sizeof(TX);
+  const uint32_t stage_bytes = x_row + (p.o ? uint32_t(blockDim.x) * 32 : 0);
+  RowTeam<kCl> t(sh, ring, p.H, p.slice, p.rows, p.teams, p.stages, p.stages * stage_bytes);
   RowExchange<kCl> row{sh.slots, sh.counts};
-  const int tid = threadIdx.x, lane = tid & 31, H = p.H;
+  const int tid = threadIdx.x, H = p.H;
   const uint32_t x_bytes = uint32_t(t.cols) * sizeof(TX), o_bytes = p.o ? uint32_t(t.cols) * 2 : 0;
-  const uint32_t stage_bytes = uint32_t(p.slice) * (sizeof(TX) + (p.o ? 2 : 0));
   ptx::pdl_wait_prior_grid();
 
   const uint64_t policy = ptx::l2_policy_evict_first();   // every row is read once
-  auto fetch = [&](int64_t r, int stage) {
+  auto fetch = [&](int r, int stage) {
     const uint32_t bar = t.bars + 8u * stage, dst = t.ring + stage * stage_bytes;
+    const int64_t at = int64_t(r) * H + t.c0;
     ptx::mbar_arrive_expect_tx(bar, x_bytes + o_bytes);
-    ptx::bulk_load(dst, static_cast<const TX*>(p.x) + r * H + t.c0, x_bytes, bar, policy);
-    if (o_bytes)
-      ptx::bulk_load(dst + uint32_t(p.slice) * sizeof(TX),
-                     static_cast<const __nv_bfloat16*>(p.o) + r * H + t.c0, o_bytes, bar, policy);
+    if (o_bytes) ptx::bulk_load(dst + x_row, static_cast<const __nv_bfloat16*>(p.o) + at, o_bytes, bar, policy);
+    ptx::bulk_load(dst, static_cast<const TX*>(p.x) + at, x_bytes, bar, policy);
   };
   if (tid == 0)
     for (int i = 0; i < p.stages && t.row0 + i < t.row1; ++i) fetch(t.row0 + i, i);
 
-  float w[16], b[kBias ? 16 : 1], cw[16], cb[kBias && kPost ? 16 : 1];
+  Row16 w, b, cw, cb;
   vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
   if constexpr (kBias) vector16(p.bias, 0, p.param_bf16, t.col, t.live, 0.f, b);
-  int64_t gate_row = -1;
+  const float quant_c = __frcp_rn(6.0f) * __frcp_rn(p.global_scale);    // quantize_kernel's estimate
+  int gate_row = -1;
   const float inv_h = 1.0f / static_cast<float>(H);
   int stage = 0;
   uint32_t phase = 0;
-  for (int64_t r = t.row0; r < t.row1; ++r) {
-    const int64_t at = r * H;
-    const int64_t g = p.gate_rows ? r / p.gate_rows : 0;
+  for (int r = t.row0; r < t.row1; ++r) {
+    const int64_t at = int64_t(r) * H;
+    const int g = p.gate_rows ? r / p.gate_rows : 0;
     if (p.o && g != gate_row) {
       gate_row = g;
-      vector16(p.gate, g * H, p.gate_bf16, t.col, t.live, 1.f, cw);
+      vector16(p.gate, int64_t(g) * H, p.gate_bf16, t.col, t.live, 1.f, cw);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) cw[i] *= p.scale;
+      for (int i = 0; i < 8; ++i) cw[i] = mul2(cw[i], both(p.scale));
       if constexpr (kPost) {
-        float v[16];
+        Row16 v;
         if constexpr (kBias) {
           vector16(p.post_bias, 0, p.param_bf16, t.col, t.live, 0.f, v);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) cb[i] = cw[i] * v[i];
+          for (int i = 0; i < 8; ++i) cb[i] = mul2(cw[i], v[i]);
         }
         vector16(p.post_weight, 0, p.param_bf16, t.col, t.live, 1.f, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) cw[i] *= v[i];
+        for (int i = 0; i < 8; ++i) cw[i] = mul2(cw[i], v[i]);
       }
     }
-    const uint32_t xs = t.ring + stage * stage_bytes, os = xs + uint32_t(p.slice) * sizeof(TX);
+    const uint32_t xs = t.ring + stage * stage_bytes;
     t.wait(stage, phase);
-    float h[16], o[16], mean_post = 0.f, rstd_post = 0.f;
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[8 * v + i] = o[8 * v + i] = 0.f;
-      if (t.live[v]) {
-        shared8<TX>(xs, t.col[v] - t.c0, h + 8 * v);
-        if (p.o) shared8<__nv_bfloat16>(os, t.col[v] - t.c0, o + 8 * v);
-      }
-    }
-    // every path below meets a barrier of the CTA after these reads, before the refill
-    auto refill = [&]() {
-      if (tid == 0 && r + p.stages < t.row1) fetch(r + p.stages, stage);
-    };
-    if (kPost) {
-      float q = 0.f;
-      if constexpr (kLayer) {
-        row.mean_squares(o, t.live, inv_h, mean_post, q);
-      } else {
-        float none = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) q = fmaf(o[i], o[i], q);
-        row.sum2(q, none, false);
-      }
-      rstd_post = __frsqrt_rn(fmaf(q, inv_h, p.eps));
-      if (blockDim.x == 32) __syncwarp();
-      refill();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[i] = t.live[i / 8] ? (o[i] - mean_post) * rstd_post : 0.f;
-    }
+    Row16 h;
+    t.template read16<TX>(xs, h);
+    float mean_post = 0.f, rstd_post = 0.f;
     if (p.o) {
+      Row16 o;
+      t.template read16<__nv_bfloat16>(xs + x_row, o);
+      if constexpr (kPost) {
+        float q;
+        if constexpr (kLayer) {
+          row.mean_squares(o, t.live, inv_h, mean_post, q);
+        } else {
+          float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) h[i] = fmaf(o[i], cw[i], h[i]);
-      if constexpr (kBias && kPost) {
+          for (int i = 0; i < 8; ++i) s = fma2(o[i], o[i], s);
+          q = row.sum(s);
+        }
+        rstd_post = rsqrtf(fmaf(q, inv_h, p.eps));
 #pragma unroll
-        for (int i = 0; i < 16; ++i) h[i] += cb[i];
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (kLayer) o[i] = add2(o[i], both(-mean_post));
+          o[i] = mul2(o[i], both(rstd_post));
+          if constexpr (kBias) h[i] = add2(h[i], cb[i]);
+        }
       }
-      if (p.h)
 #pragma unroll
-        for (int v = 0; v < 2; ++v)
-          if (t.live[v]) store8(static_cast<TX*>(p.h) + at + t.col[v], h + 8 * v);
+      for (int i = 0; i < 8; ++i) h[i] = fma2(o[i], cw[i], h[i]);
+      if (p.h) t.write16(static_cast<TX*>(p.h) + at, h);
     }
+    float mean = 0.f, q = 0.f;
     if (p.out || p.stats) {
-      float mean = 0.f, q = 0.f;
       if constexpr (kLayer) {
         row.mean_squares(h, t.live, inv_h, mean, q);
       } else {
-        float none = 0.f;
+        float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) q = fmaf(h[i], h[i], q);
-        row.sum2(q, none, false);
+        for (int i = 0; i < 8; ++i) s = fma2(h[i], h[i], s);
+        q = row.sum(s);
       }
-      if (!kPost) {
-        if (blockDim.x == 32) __syncwarp();
-        refill();
-      }
-      const float rstd = __frsqrt_rn(fmaf(q, inv_h, p.eps));
-      if (p.stats && t.rank == 0 && tid == 0)
-        reinterpret_cast<float4*>(p.stats)[r] = make_float4(mean_post, rstd_post, mean, rstd);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) h[i] = t.live[i / 8] ? (h[i] - mean) * rstd * w[i] : 0.f;
-      if constexpr (kBias) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) h[i] += t.live[i / 8] ? b[i] : 0.f;
-      }
-    } else if (!kPost) {
+      if (blockDim.x == 32) __syncwarp();
+    } else {
       t.release_barrier();
-      refill();
     }
+    // past that barrier every thread has read the stage
+    if (tid == 0 && r + p.stages < t.row1) fetch(r + p.stages, stage);
+    const float rstd = rsqrtf(fmaf(q, inv_h, p.eps));
+    if (p.stats && t.rank == 0 && tid == 0)
+      reinterpret_cast<float4*>(p.stats)[r] = make_float4(mean_post, rstd_post, mean, rstd);
     if (p.out) {
-      if (p.out_format == kOutBf16) {
 #pragma unroll
-        for (int v = 0; v < 2; ++v)
-          if (t.live[v]) store8(static_cast<__nv_bfloat16*>(p.out) + at + t.col[v], h + 8 * v);
-      } else if (p.out_format == kOutF32) {
-#pragma unroll
-        for (int v = 0; v < 2; ++v)
-          if (t.live[v]) store8(static_cast<float*>(p.out) + at + t.col[v], h + 8 * v);
-      } else {
-        uint8_t* const out = static_cast<uint8_t*>(p.out);
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const uint32_t code = quantize8(
-              h + 8 * v, t.live[v], p.out_format, p.global_scale,
-              [&](uint32_t q) {
-                if (t.live[v]) *reinterpret_cast<uint32_t*>(out + (at + t.col[v]) / 2) = q;
-              },
-              [&](uint2 q) {
-                if (t.live[v]) *reinterpret_cast<uint2*>(out + at + t.col[v]) = q;
-              });
-          // four groups' codes make one word of the row: 2 (NVFP4) or 4 lanes per group
-          const int per = p.out_format == kOutNvfp4 ? 2 : 4;
-          uint32_t word = code << (8 * ((lane / per) & 3));
-          word = (lane % per) == 0 ? word : 0u;
-          for (int k = 4 * per / 2; k > 0; k >>= 1) word |= __shfl_xor_sync(0xFFFFFFFFu, word, k);
-          if ((lane & (4 * per - 1)) == 0 && t.live[v])
-            *reinterpret_cast<uint32_t*>(
-                p.sf + sf_offset_vs(r, t.col[v] / (8 * per), H, 8 * per)) = word;
-        }
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (kLayer) h[i] = add2(h[i], both(-mean));
+        h[i] = mul2(mul2(h[i], both(rstd)), w[i]);
+        if constexpr (kBias) h[i] = add2(h[i], b[i]);
+      }
+      switch (p.out_format) {
+        case kOutBf16: t.write16(static_cast<__nv_bfloat16*>(p.out) + at, h); break;
+        case kOutF32: t.write16(static_cast<float*>(p.out) + at, h); break;
+        case kOutNvfp4: quantize_row<kOutNvfp4>(h, t, p.global_scale, quant_c, p.out, p.sf, r, H); break;
+        case kOutMxfp4: quantize_row<kOutMxfp4>(h, t, 1.f, 1.f, p.out, p.sf, r, H); break;
+        default: quantize_row<kOutMxfp8>(h, t, 1.f, 1.f, p.out, p.sf, r, H); break;
       }
     }
     if (++stage == p.stages) {
@@ -645,9 +701,10 @@ struct NormBackwardParams {
 // Backward.  With n the post-normed o (o itself without a post norm) and d = dh', a gate row's
 // sums A = sum d n and B = sum d give every gradient that the gate takes part in:
 //     dgate = scale (post_weight A + post_bias B),  dpost_weight = scale gate A, dpost_bias = scale gate B
-// so a thread keeps dweight, A (and for layer norms dbias, B) for its 16 columns, and gate, scale
-// and post weight are one vector c.  kGate: 0 no gate, 1 one gate row (sums closed once, at the
-// end), 2 several (closed at each group's last row).
+// so a thread keeps dweight, A (and where there are biases dbias, B) for its 16 columns, and gate,
+// scale and post weight are one vector c.  Over a row sum it keeps n and dh + rstd a, not a itself:
+// dh' = (dh + rstd a) - rstd [mean a] - rstd mean(a n) n.  kGate: 0 no gate, 1 one gate row (sums
+// closed once, at the end), 2 several (closed at each group's last row).
 template <class TX, int kMode, bool kPost, int kGate, int kCl>
 __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
     block_norm_backward_kernel(const __grid_constant__ NormBackwardParams p) {
@@ -656,21 +713,21 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ RowShared<kCl> sh;
   ptx::pdl_launch_dependents();
-  RowTeam<kCl> t(sh, ring, p.H, p.slice, p.rows, p.teams, p.stages);
-  RowExchange<kCl> row{sh.slots, sh.counts};
-  const int tid = threadIdx.x, H = p.H;
   // a stage: h and dh (TX), dy and o (BF16), those that are given
-  const uint32_t xs = uint32_t(p.slice) * sizeof(TX), ys = uint32_t(p.slice) * 2;
+  const uint32_t xs = uint32_t(blockDim.x) * 16 * sizeof(TX), ys = uint32_t(blockDim.x) * 32;
   const uint32_t at_dh = p.dy ? xs : 0, at_dy = at_dh + (p.dh ? xs : 0), at_o = at_dy + (p.dy ? ys : 0);
   const uint32_t stage_bytes = at_o + (p.o ? ys : 0);
+  RowTeam<kCl> t(sh, ring, p.H, p.slice, p.rows, p.teams, p.stages, p.stages * stage_bytes);
+  RowExchange<kCl> row{sh.slots, sh.counts};
+  const int tid = threadIdx.x, H = p.H;
   const uint32_t xb = uint32_t(t.cols) * sizeof(TX), yb = uint32_t(t.cols) * 2;
   const uint32_t row_bytes = (p.dy ? xb + yb : 0) + (p.dh ? xb : 0) + (p.o ? yb : 0);
   ptx::pdl_wait_prior_grid();
 
   const uint64_t policy = ptx::l2_policy_evict_first();
-  auto fetch = [&](int64_t r, int stage) {
+  auto fetch = [&](int r, int stage) {
     const uint32_t bar = t.bars + 8u * stage, dst = t.ring + stage * stage_bytes;
-    const int64_t at = r * H + t.c0;
+    const int64_t at = int64_t(r) * H + t.c0;
     ptx::mbar_arrive_expect_tx(bar, row_bytes);
     if (p.dy) {
       ptx::bulk_load(dst, static_cast<const TX*>(p.h) + at, xb, bar, policy);
@@ -682,40 +739,42 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
   if (tid == 0)
     for (int i = 0; i < p.stages && t.row0 + i < t.row1; ++i) fetch(t.row0 + i, i);
 
-  constexpr bool kRegW = !kBias;      // the bias sums leave no registers for the vectors
-  float w[kRegW ? 16 : 1], c[kRegW ? 16 : 1];
-  auto make_c = [&](int64_t g, float (&out)[16]) {
-    vector16(p.gate, g * H, p.gate_bf16, t.col, t.live, 1.f, out);
-    float v[16];
+  constexpr bool kKeep = !kBias || !kPost;    // else the sums leave no registers for the vectors
+  const float2 zero = make_float2(0.f, 0.f);
+  Row16 w, c;
+  auto make_c = [&](int g, Row16& out) {
+    vector16(kGate ? p.gate : nullptr, int64_t(g) * H, p.gate_bf16, t.col, t.live, 1.f, out);
+    Row16 v;
     if (kPost) vector16(p.post_weight, 0, p.param_bf16, t.col, t.live, 1.f, v);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) out[i] *= kPost ? p.scale * v[i] : p.scale;
+    for (int i = 0; i < 8; ++i) out[i] = mul2(out[i], kPost ? mul2(v[i], both(p.scale)) : both(p.scale));
   };
-  if constexpr (kRegW) vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
-  float dw[16], sa[16], db[kBias ? 16 : 1], sb[kBias && kPost ? 16 : 1];
-  float dwp[kGate == 2 && kPost ? 16 : 1], dbp[kGate == 2 && kPost && kBias ? 16 : 1];
+  if constexpr (kKeep) vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
+  Row16 dw, db, sa, sb, dwp, dbp;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    dw[i] = sa[i] = 0.f;
-    if constexpr (kBias) db[i] = 0.f;
-    if constexpr (kBias && kPost) sb[i] = 0.f;
-    if constexpr (kGate == 2 && kPost) dwp[i] = 0.f;
-    if constexpr (kGate == 2 && kPost && kBias) dbp[i] = 0.f;
-  }
+  for (int i = 0; i < 8; ++i) dw[i] = db[i] = sa[i] = sb[i] = dwp[i] = dbp[i] = zero;
   const int64_t vec = int64_t(p.teams) * H;           // floats of one vector's partials
-  auto store16 = [&](float* dst, const float* v) {
+  // dgate of a gate row (or a team's piece of it) from A and B
+  auto write_dgate = [&](float* dst) {
+    Row16 v, u;
+    vector16(kPost ? p.post_weight : nullptr, 0, p.param_bf16, t.col, t.live, 1.f, v);
+    if (kPost && kBias) vector16(p.post_bias, 0, p.param_bf16, t.col, t.live, 0.f, u);
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (t.live[k]) store8(dst + t.col[k], v + 8 * k);
+    for (int i = 0; i < 8; ++i) {
+      v[i] = mul2(v[i], sa[i]);
+      if constexpr (kPost && kBias) v[i] = fma2(u[i], sb[i], v[i]);
+      v[i] = mul2(v[i], both(p.scale));
+    }
+    t.write16(dst, v);
   };
   const float inv_h = 1.0f / static_cast<float>(H);
-  int64_t gate_row = -1;
+  int gate_row = -1;
   int stage = 0;
   uint32_t phase = 0;
-  for (int64_t r = t.row0; r < t.row1; ++r) {
-    const int64_t at = r * H;
-    const int64_t g = kGate == 2 ? r / p.gate_rows : 0;
-    if constexpr (kRegW) {
+  for (int r = t.row0; r < t.row1; ++r) {
+    const int64_t at = int64_t(r) * H;
+    const int g = kGate == 2 ? r / p.gate_rows : 0;
+    if constexpr (kKeep) {
       if (p.o && g != gate_row) {
         gate_row = g;
         make_c(g, c);
@@ -724,131 +783,99 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
     const float4 st = reinterpret_cast<const float4*>(p.stats)[r];
     const uint32_t base = t.ring + stage * stage_bytes;
     t.wait(stage, phase);
-    float d[16];                                      // dh', then dp
+    Row16 d;                                          // dh'
+    if (p.dh) {
+      t.template read16<TX>(base + at_dh, d);
+    } else {
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) d[8 * v + i] = 0.f;
-      if (t.live[v] && p.dh) shared8<TX>(base + at_dh, t.col[v] - t.c0, d + 8 * v);
+      for (int i = 0; i < 8; ++i) d[i] = zero;
     }
     if (p.dy) {
-      float n[16], a[16], along = 0.f, mean_a = 0.f;
+      Row16 n, a;
+      t.template read16<TX>(base, n);
+      t.template read16<__nv_bfloat16>(base + at_dy, a);
+      if constexpr (!kKeep) vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
+      float2 s = zero, sm = zero;
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) n[8 * v + i] = a[8 * v + i] = 0.f;
-        if (!t.live[v]) continue;
-        shared8<TX>(base, t.col[v] - t.c0, n + 8 * v);
-        shared8<__nv_bfloat16>(base + at_dy, t.col[v] - t.c0, a + 8 * v);
-        float wv[8];
-        if constexpr (!kRegW) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) wv[i] = 1.f;
-          if (p.weight) load8_any(p.weight, t.col[v], p.param_bf16, wv);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int k = 8 * v + i;
-          n[k] = (n[k] - st.z) * st.w;
-          dw[k] = fmaf(a[k], n[k], dw[k]);
-          if constexpr (kBias) db[k] += a[k];
-          a[k] *= kRegW ? w[kRegW ? k : 0] : wv[i];
-          along = fmaf(a[k], n[k], along);
-          if constexpr (kLayer) mean_a += a[k];
-        }
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (kLayer) n[i] = add2(n[i], both(-st.z));
+        n[i] = mul2(n[i], both(st.w));
+        dw[i] = fma2(a[i], n[i], dw[i]);
+        if constexpr (kBias) db[i] = add2(db[i], a[i]);
+        a[i] = mul2(a[i], w[i]);
+        s = fma2(a[i], n[i], s);
+        if constexpr (kLayer) sm = add2(sm, a[i]);
+        d[i] = fma2(a[i], both(st.w), d[i]);
       }
-      row.sum2(along, mean_a, kLayer);
-      along *= inv_h;
-      mean_a *= inv_h;
+      float along, mean_a = 0.f;
+      if constexpr (kLayer) row.sum2(s, sm, along, mean_a);
+      else along = row.sum(s);
+      const float2 f = both(-st.w * (along * inv_h)), m = both(-st.w * (mean_a * inv_h));
 #pragma unroll
-      for (int k = 0; k < 16; ++k)
-        d[k] = fmaf(st.w, fmaf(-n[k], along, kLayer ? a[k] - mean_a : a[k]), d[k]);
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (kLayer) d[i] = add2(d[i], m);
+        d[i] = fma2(n[i], f, d[i]);
+      }
     }
-#pragma unroll
-    for (int v = 0; v < 2; ++v)
-      if (t.live[v]) store8(static_cast<TX*>(p.dx) + at + t.col[v], d + 8 * v);
-    float n[16];
+    t.write16(static_cast<TX*>(p.dx) + at, d);
+    Row16 n;
     if (p.o) {
+      t.template read16<__nv_bfloat16>(base + at_o, n);
+      if constexpr (!kKeep) make_c(g, c);
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) n[8 * v + i] = 0.f;
-        if (!t.live[v]) continue;
-        shared8<__nv_bfloat16>(base + at_o, t.col[v] - t.c0, n + 8 * v);
-        float cv[8];
-        if constexpr (!kRegW) {
-          float pw[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) cv[i] = pw[i] = 1.f;
-          if (kGate) load8_any(p.gate, g * H + t.col[v], p.gate_bf16, cv);
-          if (kPost && p.post_weight) load8_any(p.post_weight, t.col[v], p.param_bf16, pw);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) cv[i] *= p.scale * pw[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int k = 8 * v + i;
-          if constexpr (kPost) n[k] = (n[k] - st.x) * st.y;
-          if (kPost || kGate) sa[k] = fmaf(d[k], n[k], sa[k]);
-          if constexpr (kBias && kPost) sb[k] += d[k];
-          d[k] *= kRegW ? c[kRegW ? k : 0] : cv[i];
-        }
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (kPost && kLayer) n[i] = add2(n[i], both(-st.x));
+        if constexpr (kPost) n[i] = mul2(n[i], both(st.y));
+        if constexpr (kPost || kGate) sa[i] = fma2(d[i], n[i], sa[i]);
+        if constexpr (kPost && kBias) sb[i] = add2(sb[i], d[i]);
+        d[i] = mul2(d[i], c[i]);
       }
     }
-    if (kPost) {
-      float along = 0.f, mean_a = 0.f;
+    if constexpr (kPost) {
+      float2 s = zero, sm = zero;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        along = fmaf(t.live[k / 8] ? d[k] : 0.f, n[k], along);
-        if constexpr (kLayer) mean_a += t.live[k / 8] ? d[k] : 0.f;
+      for (int i = 0; i < 8; ++i) {
+        s = fma2(d[i], n[i], s);
+        if constexpr (kLayer) sm = add2(sm, d[i]);
       }
-      row.sum2(along, mean_a, kLayer);
+      float along, mean_a = 0.f;
+      if constexpr (kLayer) row.sum2(s, sm, along, mean_a);
+      else along = row.sum(s);
       if (blockDim.x == 32) __syncwarp();
-      along *= inv_h;
-      mean_a *= inv_h;
+      const float2 f = both(-(along * inv_h)), m = both(-(mean_a * inv_h));
 #pragma unroll
-      for (int k = 0; k < 16; ++k)
-        d[k] = st.y * fmaf(-n[k], along, kLayer ? d[k] - mean_a : d[k]);
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (kLayer) d[i] = add2(d[i], m);
+        d[i] = mul2(fma2(n[i], f, d[i]), both(st.y));
+      }
     } else {
-      t.release_barrier();                            // every thread has read the stage
+      t.release_barrier();
     }
+    // past that barrier every thread has read the stage
     if (tid == 0 && r + p.stages < t.row1) fetch(r + p.stages, stage);
-    if (p.o)
-#pragma unroll
-      for (int v = 0; v < 2; ++v)
-        if (t.live[v]) store8(static_cast<__nv_bfloat16*>(p.d_o) + at + t.col[v], d + 8 * v);
+    if (p.o) t.write16(static_cast<__nv_bfloat16*>(p.d_o) + at, d);
 
     if constexpr (kGate == 2) {
-      const int64_t g0 = g * p.gate_rows, g1 = min(int64_t(p.rows), g0 + p.gate_rows);
+      const int64_t g0 = int64_t(g) * p.gate_rows, g1 = min(int64_t(p.rows), g0 + p.gate_rows);
       if (r + 1 == t.row1 || r + 1 == g1) {
         // close the group's sums in this team: the whole group's (stored), or an edge piece for
         // the second kernel: slot 0 if the group began in an earlier team, else slot 1
-        if (p.dgate) {
-          float v[16], u[16];
-          vector16(kPost ? p.post_weight : nullptr, 0, p.param_bf16, t.col, t.live, 1.f, v);
-          vector16(kPost && kBias ? p.post_bias : nullptr, 0, p.param_bf16, t.col, t.live, 0.f, u);
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            v[k] *= p.scale * sa[k];
-            if constexpr (kBias && kPost) v[k] = fmaf(p.scale * u[k], sb[k], v[k]);
-          }
-          store16(g0 >= t.row0 && g1 <= t.row1 ? p.dgate + g * H
-                                               : p.ws + (g0 < t.row0 ? 4 : 5) * vec + int64_t(t.team) * H, v);
-        }
+        if (p.dgate)
+          write_dgate(g0 >= t.row0 && g1 <= t.row1
+                          ? p.dgate + int64_t(g) * H
+                          : p.ws + (g0 < t.row0 ? 4 : 5) * vec + int64_t(t.team) * H);
         if constexpr (kPost) {
-          float v[16];
-          vector16(p.gate, g * H, p.gate_bf16, t.col, t.live, 1.f, v);
+          Row16 v;
+          vector16(p.gate, int64_t(g) * H, p.gate_bf16, t.col, t.live, 1.f, v);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            dwp[k] = fmaf(p.scale * v[k], sa[k], dwp[k]);
-            if constexpr (kBias) dbp[k] = fmaf(p.scale * v[k], sb[k], dbp[k]);
+          for (int i = 0; i < 8; ++i) {
+            v[i] = mul2(v[i], both(p.scale));
+            dwp[i] = fma2(v[i], sa[i], dwp[i]);
+            if constexpr (kBias) dbp[i] = fma2(v[i], sb[i], dbp[i]);
           }
         }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          sa[k] = 0.f;
-          if constexpr (kBias && kPost) sb[k] = 0.f;
-        }
+        for (int i = 0; i < 8; ++i) sa[i] = sb[i] = zero;
       }
     }
     if (++stage == p.stages) {
@@ -857,37 +884,24 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
     }
   }
   float* const mine = p.ws + int64_t(t.team) * H;
-  if (p.dweight) store16(mine, dw);
-  if constexpr (kBias)
-    if (p.dbias) store16(mine + vec, db);
-  if constexpr (kGate == 2 && kPost) {
-    if (p.dpost_weight) store16(mine + 2 * vec, dwp);
-    if constexpr (kBias)
-      if (p.dpost_bias) store16(mine + 3 * vec, dbp);
-  } else if constexpr (kPost || kGate == 1) {
-    float gv[16];
-    vector16(kGate ? p.gate : nullptr, 0, p.gate_bf16, t.col, t.live, 1.f, gv);
-    if (kGate && p.dgate) {          // the only group; a team's piece of it (slot 1 of the first)
-      float v[16], u[16];
-      vector16(kPost ? p.post_weight : nullptr, 0, p.param_bf16, t.col, t.live, 1.f, v);
-      vector16(kPost && kBias ? p.post_bias : nullptr, 0, p.param_bf16, t.col, t.live, 0.f, u);
+  if (p.dweight) t.write16(mine, dw);
+  if (kBias && p.dbias) t.write16(mine + vec, db);
+  if constexpr (kGate == 1) {          // the only group; a team's piece of it (slot 1 of the first)
+    if (p.dgate) write_dgate(p.teams == 1 ? p.dgate : mine + (t.team ? 4 : 5) * vec);
+  }
+  if constexpr (kPost) {
+    if constexpr (kGate != 2) {
+      Row16 v;
+      vector16(kGate ? p.gate : nullptr, 0, p.gate_bf16, t.col, t.live, 1.f, v);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        v[k] *= p.scale * sa[k];
-        if constexpr (kBias && kPost) v[k] = fmaf(p.scale * u[k], sb[k], v[k]);
-      }
-      store16(p.teams == 1 ? p.dgate : mine + (t.team ? 4 : 5) * vec, v);
-    }
-    if constexpr (kPost) {
-#pragma unroll
-      for (int k = 0; k < 16; ++k) sa[k] *= p.scale * gv[k];
-      if (p.dpost_weight) store16(mine + 2 * vec, sa);
-      if constexpr (kBias) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) sb[k] *= p.scale * gv[k];
-        if (p.dpost_bias) store16(mine + 3 * vec, sb);
+      for (int i = 0; i < 8; ++i) {
+        v[i] = mul2(v[i], both(p.scale));
+        dwp[i] = mul2(v[i], sa[i]);
+        dbp[i] = mul2(v[i], sb[i]);
       }
     }
+    if (p.dpost_weight) t.write16(mine + 2 * vec, dwp);
+    if (kBias && p.dpost_bias) t.write16(mine + 3 * vec, dbp);
   }
   if constexpr (kCl > 1) ptx::cluster_sync();
 #endif
@@ -944,7 +958,7 @@ inline cudaError_t launch_block_norm(NormParams& p, bool post, cudaStream_t s) {
   const Geometry g = geometry(p.H);
   auto* kernel = g.cluster == 1 ? (post ? block_norm_kernel<TX, kMode, true, 1> : block_norm_kernel<TX, kMode, false, 1>)
                                 : (post ? block_norm_kernel<TX, kMode, true, 2> : block_norm_kernel<TX, kMode, false, 2>);
-  return launch_rows(kernel, p, g, g.slice * int(sizeof(TX) + (p.o ? 2 : 0)), s);
+  return launch_rows(kernel, p, g, 16 * g.threads * int(sizeof(TX) + (p.o ? 2 : 0)), s);
 }
 
 template <class TX, int kMode, bool kPost, int kGate>
@@ -953,7 +967,7 @@ inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, cudaStream_
   auto* kernel = g.cluster == 1 ? block_norm_backward_kernel<TX, kMode, kPost, kGate, 1>
                                 : block_norm_backward_kernel<TX, kMode, kPost, kGate, 2>;
   const int per = (p.dy ? int(sizeof(TX)) + 2 : 0) + (p.dh ? int(sizeof(TX)) : 0) + (p.o ? 2 : 0);
-  return launch_rows(kernel, p, g, g.slice * per, s);
+  return launch_rows(kernel, p, g, 16 * g.threads * per, s);
 }
 template <class TX, int kMode, bool kPost>
 inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, int gate, cudaStream_t s) {
