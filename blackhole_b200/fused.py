@@ -9,9 +9,9 @@ are).  Calls are asynchronous on `stream`, the current stream by default.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
-from . import SCHEDULES, BlackholeError, _ptr, _stream, load
+from . import SCHEDULES, BlackholeError, _ptr, load
 
 __all__ = ["ACTIVATIONS", "nvfp4_bf16_gemm_fused", "mxfp4_bf16_gemm_fused", "mxf8f4_bf16_gemm_fused",
            "gemm_fused_backward", "gemm_fused_backward_workspace_bytes", "NORM_KINDS", "NORM_OUTPUTS", "block_norm", "block_norm_backward",
@@ -21,77 +21,67 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 NORM_KINDS = {"rms": 0, "layer": 1}
 NORM_OUTPUTS = {"bf16": 0, "f32": 1, "nvfp4": 2, "mxfp4": 3, "mxfp8": 4}
 
-_vp, _i32, _f32, _i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
+
+# The C structs of include/blackhole_sm100.h, in their field order (native alignment); a call packs
+# its arguments into bytes and passes their address.
+_EPILOGUE = struct.Struct("@3if3P")             # blackhole_sm100_epilogue
+_NORM = struct.Struct("@9i3f11P")               # blackhole_sm100_block_norm_args
+_NORM_BACKWARD = struct.Struct("@8if17Pq")      # blackhole_sm100_block_norm_backward_args
+
+_torch = None
 
 
-class Epilogue(ctypes.Structure):
-    """blackhole_sm100_epilogue"""
-    _fields_ = [(n, _i32) for n in ("activation", "gated", "bias_is_bf16")] + [("beta", _f32)] + \
-               [(n, _vp) for n in ("bias", "residual", "Z")]
+def _device():
+    """torch, and the current CUDA device (-1 without one: raw pointers can still be passed)."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch.cuda.current_device() if _torch.cuda.is_initialized() or _torch.cuda.is_available() else -1
 
 
-class BlockNormArgs(ctypes.Structure):
-    """blackhole_sm100_block_norm_args"""
-    _fields_ = [(n, _i32) for n in ("rows", "H", "kind", "x_is_bf16", "param_is_bf16", "gate_is_bf16",
-                                    "post_norm", "gate_rows", "out_format")] + \
-               [(n, _f32) for n in ("eps", "scale", "global_scale")] + \
-               [(n, _vp) for n in ("x", "o", "gate", "weight", "bias", "post_weight", "post_bias",
-                                   "h", "out", "sf", "stats")]
+def _handle(stream, device):
+    if stream is None:
+        return _torch.cuda.current_stream(device).cuda_stream if device >= 0 else 0
+    if type(stream) is int:
+        return stream
+    if stream.device.index != device:
+        raise ValueError(f"stream is on {stream.device}, the current device is cuda:{device}")
+    return stream.cuda_stream
 
 
-class BlockNormBackwardArgs(ctypes.Structure):
-    """blackhole_sm100_block_norm_backward_args"""
-    _fields_ = [(n, _i32) for n in ("rows", "H", "kind", "x_is_bf16", "param_is_bf16", "gate_is_bf16",
-                                    "post_norm", "gate_rows")] + [("scale", _f32)] + \
-               [(n, _vp) for n in ("h", "dy", "dh", "o", "gate", "weight", "post_weight", "post_bias",
-                                   "stats", "dx", "d_o", "dweight", "dbias", "dpost_weight",
-                                   "dpost_bias", "dgate", "workspace")] + \
-               [("workspace_bytes", _i64)]
+def _at(name, t, numel, dtype, device):
+    """The address of a tensor that fits (or the raw pointer, or 0 for None)."""
+    if t is None:
+        return 0
+    if type(t) is int:
+        return t
+    try:
+        if t.dtype is dtype and t.numel() >= numel and t.get_device() == device and t.is_contiguous() and device >= 0:
+            return t.data_ptr()
+    except AttributeError:
+        raise TypeError(f"{name}: cannot take a device pointer from {type(t)!r}") from None
+    if not t.is_cuda:
+        raise ValueError(f"{name}: tensor must live on a CUDA device")
+    if t.get_device() != device:
+        raise ValueError(f"{name}: tensor is on {t.device}, the current device is cuda:{device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: tensor must be contiguous")
+    if t.dtype is not dtype:
+        raise ValueError(f"{name}: {t.dtype}, {dtype} is wanted (tensors of one kind share a type)")
+    raise ValueError(f"{name}: {t.numel()} elements, {numel} are needed")
 
 
-def _torch():
-    import torch
-    return torch
-
-
-class _Buffers:
-    """Checks a call's tensors and gives their addresses.  Tensors of one `kind` (the stream, the
-    parameters, the gate) share a type, BF16 or FP32."""
-
-    def __init__(self, stream):
-        self.torch = _torch()
-        self.device = self.torch.cuda.current_device() if self.torch.cuda.is_available() else -1
-        if stream is not None and getattr(stream, "device", None) is not None \
-                and stream.device.index != self.device:
-            raise ValueError(f"stream is on {stream.device}, the current device is cuda:{self.device}")
-        self.kinds = {}
-
-    def __call__(self, name, t, numel, dtype=None, kind=None):
-        if t is None or type(t) is int:
-            return t
-        if not hasattr(t, "data_ptr"):
-            raise TypeError(f"{name}: cannot take a device pointer from {type(t)!r}")
-        if not t.is_cuda:
-            raise ValueError(f"{name}: tensor must live on a CUDA device")
-        if t.get_device() != self.device:
-            raise ValueError(f"{name}: tensor is on cuda:{t.get_device()}, the current device is cuda:{self.device}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name}: tensor must be contiguous")
-        if t.numel() < numel:
-            raise ValueError(f"{name}: {t.numel()} elements, {numel} are needed")
-        if kind is not None:
-            if self.kinds.setdefault(kind, t.dtype) != t.dtype:
-                raise ValueError(f"{name}: {t.dtype}, but another tensor of its kind has {self.kinds[kind]}")
-            if t.dtype not in (self.torch.bfloat16, self.torch.float32):
-                raise ValueError(f"{name}: {t.dtype}, torch.bfloat16 or torch.float32 is wanted")
-        elif t.dtype != dtype:
-            raise ValueError(f"{name}: {t.dtype}, {dtype} is wanted")
-        return t.data_ptr()
-
-    def is_bf16(self, kind, told):
-        """1 if the kind's tensors are BF16; for raw pointers what the caller says."""
-        dtype = self.kinds.get(kind)
-        return int(told if dtype is None else dtype == self.torch.bfloat16)
+def _kind(told_bf16, *tensors):
+    """The type of a call's tensors of one kind (the stream, the parameters, the gate): that of the
+    first one given, BF16 or FP32; for raw pointers what the caller says."""
+    for t in tensors:
+        dtype = getattr(t, "dtype", None)
+        if dtype is not None:
+            if dtype is not _torch.bfloat16 and dtype is not _torch.float32:
+                raise ValueError(f"{dtype}: torch.bfloat16 or torch.float32 is wanted")
+            return dtype
+    return _torch.bfloat16 if told_bf16 else _torch.float32
 
 
 def _gate_elements(rows, H, gate_rows):
@@ -104,20 +94,19 @@ def _blocked_bytes(rows, H, vec):
 
 def _gemm_fused(name, M, N, K, A, SFA, B, SFB, D, alpha, bias, activation, gated, residual, beta, Z,
                 bias_is_bf16, schedule, workspace, workspace_bytes, stream):
-    M, N = int(M), int(N)
-    b = _Buffers(stream)
-    bf16 = b.torch.bfloat16
-    n_out = N // 2 if gated else N
-    p_d, p_res, p_z = b("D", D, M * n_out, bf16), b("residual", residual, M * n_out, bf16), b("Z", Z, M * N, bf16)
-    p_bias = b("bias", bias, N, kind="bias")
+    dev = _device()
+    handle, bf16 = _handle(stream, dev), _torch.bfloat16
+    n = M * (N // 2 if gated else N)
+    t_bias = _kind(bias_is_bf16, bias)
+    epi = _EPILOGUE.pack(ACTIVATIONS[activation], 1 if gated else 0, t_bias is bf16, beta,
+                         _at("bias", bias, N, t_bias, dev), _at("residual", residual, n, bf16, dev),
+                         _at("Z", Z, M * N, bf16, dev))
     if workspace is not None and hasattr(workspace, "numel") and not workspace_bytes:
         workspace_bytes = workspace.numel() * workspace.element_size()
-    epi = Epilogue(ACTIVATIONS[activation], int(bool(gated)), b.is_bf16("bias", bias_is_bf16), beta,
-                   p_bias, p_res, p_z)
-    rc = getattr(load(), name)(M, N, int(K), _ptr(A), _ptr(SFA), _ptr(B), _ptr(SFB), p_d, alpha,
-                               ctypes.byref(epi), SCHEDULES[schedule],
+    rc = getattr(load(), name)(M, N, K, _ptr(A), _ptr(SFA), _ptr(B), _ptr(SFB),
+                               _at("D", D, n, bf16, dev), alpha, epi, SCHEDULES[schedule],
                                _ptr(workspace) if workspace is not None else None,
-                               int(workspace_bytes), _stream(stream))
+                               workspace_bytes, handle)
     if rc != 0:
         raise BlackholeError(name, rc)
 
@@ -177,21 +166,15 @@ def gemm_fused_backward(M: int, N: int, dD, Z, dZ, dbias=None, activation: str =
     dD: BF16 of D's shape.  dZ may be Z, or dD when not gated.  workspace:
     gemm_fused_backward_workspace_bytes bytes, or None: allocated for this call from torch's
     caching allocator on the current stream."""
-    M, N = int(M), int(N)
-    b = _Buffers(stream)
-    bf16 = b.torch.bfloat16
-    p_d, p_z, p_dz = b("dD", dD, M * (N // 2 if gated else N), bf16), b("Z", Z, M * N, bf16), b("dZ", dZ, M * N, bf16)
-    p_db = b("dbias", dbias, N, b.torch.float32)
-    if workspace is None and p_db:
-        need = gemm_fused_backward_workspace_bytes(M, N)
-        if need > 0:
-            workspace = _workspace(b, need, stream)
-    if workspace is not None and type(workspace) is not int:
-        workspace_bytes = workspace.numel() * workspace.element_size()
-        workspace = b("workspace", workspace, 0, workspace.dtype)
-    rc = load().blackhole_sm100_gemm_fused_backward(M, N, p_d, p_z, p_dz, p_db, ACTIVATIONS[activation],
-                                                    int(bool(gated)), workspace, int(workspace_bytes),
-                                                    _stream(stream))
+    dev = _device()
+    handle, bf16 = _handle(stream, dev), _torch.bfloat16
+    p_db = _at("dbias", dbias, N, _torch.float32, dev)
+    need = gemm_fused_backward_workspace_bytes(M, N) if p_db and workspace is None else 0
+    p_ws, workspace_bytes, workspace = _scratch(workspace, workspace_bytes, need, stream, dev)
+    rc = load().blackhole_sm100_gemm_fused_backward(
+        M, N, _at("dD", dD, M * (N // 2 if gated else N), bf16, dev), _at("Z", Z, M * N, bf16, dev),
+        _at("dZ", dZ, M * N, bf16, dev), p_db, ACTIVATIONS[activation], 1 if gated else 0, p_ws,
+        workspace_bytes, handle)
     if rc != 0:
         raise BlackholeError("blackhole_sm100_gemm_fused_backward", rc)
 
@@ -217,25 +200,23 @@ def block_norm(rows: int, H: int, x, out=None, weight=None, bias=None, kind: str
     4 FP32) keeps what block_norm_backward needs.  The *_is_bf16 flags only matter for raw
     pointers.  rows >= 1, H % 8 == 0 (NVFP4 16, MX 32), H <= 16384.
     Raises ValueError for tensors that do not fit, BlackholeError for what the library refuses."""
-    rows, H = int(rows), int(H)
-    fmt = NORM_OUTPUTS[out_format]
-    b = _Buffers(stream)
-    bf16, f32, u8 = b.torch.bfloat16, b.torch.float32, b.torch.uint8
-    n = rows * H
+    dev = _device()
+    handle, fmt, n = _handle(stream, dev), NORM_OUTPUTS[out_format], rows * H
+    bf16, f32, u8 = _torch.bfloat16, _torch.float32, _torch.uint8
     out_n, out_t = ((n, bf16), (n, f32), (n // 2, u8), (n // 2, u8), (n, u8))[fmt]
-    p_x, p_h = b("x", x, n, kind="x"), b("h", h, n, kind="x")
-    p_o = b("o", o, n, bf16)
-    p_gate = b("gate", gate, _gate_elements(rows, H, gate_rows), kind="gate")
-    p_w, p_b = b("weight", weight, H, kind="param"), b("bias", bias, H, kind="param")
-    p_pw, p_pb = b("post_weight", post_weight, H, kind="param"), b("post_bias", post_bias, H, kind="param")
-    p_out = b("out", out, out_n, out_t)
-    p_sf = b("sf", sf, _blocked_bytes(rows, H, 16 if fmt == 2 else 32), u8)
-    p_st = b("stats", stats, 4 * rows, f32)
-    args = BlockNormArgs(rows, H, NORM_KINDS[kind], b.is_bf16("x", x_is_bf16),
-                         b.is_bf16("param", param_is_bf16), b.is_bf16("gate", gate_is_bf16),
-                         int(post_norm), int(gate_rows), fmt, eps, scale, global_scale,
-                         p_x, p_o, p_gate, p_w, p_b, p_pw, p_pb, p_h, p_out, p_sf, p_st)
-    rc = load().blackhole_sm100_block_norm(ctypes.byref(args), _stream(stream))
+    tx, tp, tg = (_kind(x_is_bf16, x), _kind(param_is_bf16, weight, bias, post_weight, post_bias),
+                  _kind(gate_is_bf16, gate))
+    args = _NORM.pack(
+        rows, H, NORM_KINDS[kind], tx is bf16, tp is bf16, tg is bf16, bool(post_norm), gate_rows, fmt,
+        eps, scale, global_scale,
+        _at("x", x, n, tx, dev), _at("o", o, n, bf16, dev),
+        _at("gate", gate, _gate_elements(rows, H, gate_rows), tg, dev),
+        _at("weight", weight, H, tp, dev), _at("bias", bias, H, tp, dev),
+        _at("post_weight", post_weight, H, tp, dev), _at("post_bias", post_bias, H, tp, dev),
+        _at("h", h, n, tx, dev), _at("out", out, out_n, out_t, dev),
+        _at("sf", sf, _blocked_bytes(rows, H, 16 if fmt == 2 else 32), u8, dev),
+        _at("stats", stats, 4 * rows, f32, dev))
+    rc = load().blackhole_sm100_block_norm(args, handle)
     if rc != 0:
         raise BlackholeError("blackhole_sm100_block_norm", rc)
 
@@ -260,44 +241,45 @@ def block_norm_backward(rows: int, H: int, h, stats, dx, dy=None, dh=None, weigh
     dpost_bias (H FP32 values) and dgate (FP32, gate's shape): overwritten where given.
     workspace: block_norm_backward_workspace_bytes bytes, or None: allocated for this call from
     torch's caching allocator on the current stream."""
-    rows, H = int(rows), int(H)
-    b = _Buffers(stream)
-    bf16, f32 = b.torch.bfloat16, b.torch.float32
-    n = rows * H
-    p_h, p_st = b("h", h, n, kind="x"), b("stats", stats, 4 * rows, f32)
-    p_dy, p_dh = b("dy", dy, n, bf16), b("dh", dh, n, kind="x")
-    p_o, p_do, p_dx = b("o", o, n, bf16), b("do", do, n, bf16), b("dx", dx, n, kind="x")
-    g_n = _gate_elements(rows, H, gate_rows)
-    p_gate, p_dgate = b("gate", gate, g_n, kind="gate"), b("dgate", dgate, g_n, f32)
-    p_w = b("weight", weight, H, kind="param")
-    p_pw, p_pb = b("post_weight", post_weight, H, kind="param"), b("post_bias", post_bias, H, kind="param")
-    p_dw, p_db = b("dweight", dweight, H, f32), b("dbias", dbias, H, f32)
-    p_dpw, p_dpb = b("dpost_weight", dpost_weight, H, f32), b("dpost_bias", dpost_bias, H, f32)
-    sums = p_dw or p_db or p_dpw or p_dpb or (p_dgate and gate_rows != 1)
-    if workspace is None and sums:
+    dev = _device()
+    handle, n, g_n = _handle(stream, dev), rows * H, _gate_elements(rows, H, gate_rows)
+    bf16, f32 = _torch.bfloat16, _torch.float32
+    tx, tp, tg = (_kind(x_is_bf16, h), _kind(param_is_bf16, weight, post_weight, post_bias),
+                  _kind(gate_is_bf16, gate))
+    sums = [_at("dweight", dweight, H, f32, dev), _at("dbias", dbias, H, f32, dev),
+            _at("dpost_weight", dpost_weight, H, f32, dev), _at("dpost_bias", dpost_bias, H, f32, dev),
+            _at("dgate", dgate, g_n, f32, dev)]
+    need = 0
+    if workspace is None and (any(sums[:4]) or (sums[4] and gate_rows != 1)):
         need = block_norm_backward_workspace_bytes(rows, H, gate is not None, gate_rows)
-        if need > 0:
-            workspace = _workspace(b, need, stream)
-    if workspace is not None and type(workspace) is not int:
-        workspace_bytes = workspace.numel() * workspace.element_size()
-        workspace = b("workspace", workspace, 0, workspace.dtype)
-    args = BlockNormBackwardArgs(rows, H, NORM_KINDS[kind], b.is_bf16("x", x_is_bf16),
-                                 b.is_bf16("param", param_is_bf16), b.is_bf16("gate", gate_is_bf16),
-                                 int(post_norm), int(gate_rows), scale, p_h, p_dy, p_dh, p_o, p_gate,
-                                 p_w, p_pw, p_pb, p_st, p_dx, p_do, p_dw, p_db, p_dpw, p_dpb, p_dgate,
-                                 workspace, int(workspace_bytes))
-    rc = load().blackhole_sm100_block_norm_backward(ctypes.byref(args), _stream(stream))
+    p_ws, workspace_bytes, workspace = _scratch(workspace, workspace_bytes, need, stream, dev)
+    args = _NORM_BACKWARD.pack(
+        rows, H, NORM_KINDS[kind], tx is bf16, tp is bf16, tg is bf16, bool(post_norm), gate_rows, scale,
+        _at("h", h, n, tx, dev), _at("dy", dy, n, bf16, dev), _at("dh", dh, n, tx, dev),
+        _at("o", o, n, bf16, dev), _at("gate", gate, g_n, tg, dev), _at("weight", weight, H, tp, dev),
+        _at("post_weight", post_weight, H, tp, dev), _at("post_bias", post_bias, H, tp, dev),
+        _at("stats", stats, 4 * rows, f32, dev), _at("dx", dx, n, tx, dev), _at("do", do, n, bf16, dev),
+        *sums, p_ws, workspace_bytes)
+    rc = load().blackhole_sm100_block_norm_backward(args, handle)
     if rc != 0:
         raise BlackholeError("blackhole_sm100_block_norm_backward", rc)
 
 
-def _workspace(b, nbytes, stream):
-    """Scratch for one call on `stream`: memory the allocator hands out again only after the
-    work enqueued there."""
-    torch = b.torch
-    if stream is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=b.device)
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
-    with torch.cuda.stream(stream):
-        return torch.empty(nbytes, dtype=torch.uint8, device=b.device)
+def _scratch(workspace, workspace_bytes, need, stream, device):
+    """(address, bytes, owner) of a call's workspace: the caller's, or `need` bytes of torch's
+    caching allocator on `stream`, which hands them out again only after the work enqueued there."""
+    if workspace is None:
+        if need <= 0 or device < 0:
+            return 0, 0, None
+        if stream is None:
+            workspace = _torch.empty(need, dtype=_torch.uint8, device=device)
+        else:
+            if type(stream) is int:
+                stream = _torch.cuda.ExternalStream(stream) if stream else _torch.cuda.default_stream()
+            with _torch.cuda.stream(stream):
+                workspace = _torch.empty(need, dtype=_torch.uint8, device=device)
+        return workspace.data_ptr(), need, workspace
+    if type(workspace) is int:
+        return workspace, workspace_bytes, workspace
+    return (_at("workspace", workspace, 0, workspace.dtype, device),
+            workspace.numel() * workspace.element_size(), workspace)

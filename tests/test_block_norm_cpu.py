@@ -1,6 +1,4 @@
 """What the block norm calls refuse, before any device work (no GPU needed)."""
-import ctypes
-
 import pytest
 
 import blackhole_b200 as bh
@@ -66,11 +64,10 @@ def test_names_and_null_arguments():
     L = bh.load()
     assert L.blackhole_sm100_block_norm(None, None) == 1
     assert L.blackhole_sm100_block_norm_backward(None, None) == 1
-    bad = fused.BlockNormArgs(4, 256, 2, 1, 0, 1, 0, 0, 0, 1e-6, 1.0, 1.0, A, None, None, None, None, None, None,
-                              None, A + STEP, None, None)
-    assert L.blackhole_sm100_block_norm(ctypes.byref(bad), None) == 1        # kind 2
-    bad.kind, bad.out_format = 0, 5
-    assert L.blackhole_sm100_block_norm(ctypes.byref(bad), None) == 1
+    ptrs = [A] + [0] * 7 + [A + STEP, 0, 0]
+    pack = lambda kind, fmt: fused._NORM.pack(4, 256, kind, 1, 0, 1, 0, 0, fmt, 1e-6, 1.0, 1.0, *ptrs)  # noqa: E731
+    for kind, fmt in ((2, 0), (-1, 0), (0, 5), (0, -1)):
+        assert L.blackhole_sm100_block_norm(pack(kind, fmt), None) == 1
 
 
 def test_tensors_are_checked():

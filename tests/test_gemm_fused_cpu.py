@@ -2,6 +2,7 @@
 import pytest
 
 import blackhole_b200 as bh
+from blackhole_b200.fused import _EPILOGUE
 
 A = 1 << 40          # aligned addresses that are never dereferenced: every case is refused first
 S = 1 << 34
@@ -45,12 +46,10 @@ def test_names_and_null_epilogue():
         fn = getattr(L, f"blackhole_sm100_{f}_bf16_gemm_fused")
         args = (16, 256, 256, A, A + S, A + 2 * S, A + 3 * S, A + 4 * S, 1.0)
         assert fn(*args, None, 0, None, 0, None) == 1
-        import ctypes
-        from blackhole_b200.fused import Epilogue
         for sched in (-1, 5):
-            assert fn(*args, ctypes.byref(Epilogue(0, 0, 0, 1.0, None, None, None)), sched, None, 0, None) == 1
+            assert fn(*args, _EPILOGUE.pack(0, 0, 0, 1.0, 0, 0, 0), sched, None, 0, None) == 1
         for act in (-1, 5):
-            assert fn(*args, ctypes.byref(Epilogue(act, 0, 0, 1.0, None, None, None)), 0, None, 0, None) == 1
+            assert fn(*args, _EPILOGUE.pack(act, 0, 0, 1.0, 0, 0, 0), 0, None, 0, None) == 1
 
 
 @pytest.mark.parametrize("over", [
