@@ -21,6 +21,7 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC,-fvisibility=hidden",
     "-Xptxas", "-v",
     "--expt-relaxed-constexpr",
+    "-split-compile=0",
     "-shared",
 ]
 

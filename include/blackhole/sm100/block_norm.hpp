@@ -37,6 +37,7 @@
 
 #include <blackhole/common/sf_layout.hpp>
 #include <blackhole/sm100/column_sum.hpp>
+#include <blackhole/sm100/f32x2.hpp>
 #include <blackhole/sm100/gemm_epilogue.hpp>
 #include <blackhole/sm100/nvfp4_gemm_common.hpp>
 #include <blackhole/sm100/nvfp4_quant.hpp>
@@ -187,35 +188,16 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Pairs of FP32 values, as sm_100's packed FP32 instructions take them: half the issue slots of
-// one value at a time (these kernels were bound by instruction issue before).
-__device__ __forceinline__ uint64_t pair_bits(float2 v) { return (uint64_t(__float_as_uint(v.y)) << 32) | __float_as_uint(v.x); }
-__device__ __forceinline__ float2 pair_of(uint64_t b) {
-  return make_float2(__uint_as_float(uint32_t(b)), __uint_as_float(uint32_t(b >> 32)));
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
-  return pair_of(d);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
-  return pair_of(d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
-  return pair_of(d);
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// Pair arithmetic (f32x2.hpp): these kernels were bound by instruction issue before.
+using detail::add2;
+using detail::both;
+using detail::fma2;
+using detail::mul2;
+using detail::unpack2;
 
 // A thread's 16 columns of a row, as 8 pairs: pairs 0-3 its first 8-column vector, 4-7 its second.
 using Row16 = float2[8];
 
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
 // 8 values at element `at` of a row in shared memory.
 template <class T>
 __device__ __forceinline__ void shared8(uint32_t row, int at, float2* v) {

@@ -21,11 +21,14 @@
 #include <cuda_runtime_api.h>
 
 #include <blackhole/sm100/column_sum.hpp>
+#include <blackhole/sm100/f32x2.hpp>
 #include <blackhole/sm100/nvfp4_gemm_common.hpp>
 #include <blackhole_sm100.h>
 
 namespace blackhole::sm100 {
 
+// (kNoEpilogue: a kernel without one.)
+constexpr int kNoEpilogue = -1;
 enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
 
 namespace detail {
@@ -56,56 +59,134 @@ inline cudaError_t epilogue_check_args(int M, int N, const void* D,
   return cudaSuccess;
 }
 
+// Warp roles of the tiled schedules with an epilogue: 4 control warps (TMA, MMA, scale-factor
+// copies, one idle) and 8 epilogue warps, so that registers can be split by warpgroup: an epilogue
+// warp holds a row's 128 accumulators, the residual fetched ahead and the activation's temporaries,
+// which at an even split (168 each) spilled 0.4-1.1 KB per thread.
+template <class Base>
+struct FusedTraits : Base {
+  static constexpr bool RegSplit = true;
+  static constexpr int NumWarps = 12;
+  static constexpr int NumThreads = NumWarps * 32;
+  static constexpr int FirstEpiWarp = 4;
+  static constexpr int SfWarp = 2;
+  static constexpr int ControlRegs = 64;
+  static constexpr int EpiRegs = 208;
+  static constexpr int MinRegs = (ControlRegs * 128 + EpiRegs * 256 + NumThreads - 1) / NumThreads;   // 160
+  static_assert(Base::NumEpiWarps == 8, "two warpgroups of epilogue warps");
+};
+
 #if defined(__CUDACC__)
 
 namespace detail {
 
-// ---- activations --------------------------------------------------------------------------
-// exp and the divisions below are the fast forms (relative error a few 2^-23, against the 2^-9 of
-// the BF16 result); every form keeps its relative accuracy in the tails, where 1 + tanh or 1 + erf
-// would cancel.  |z| past 30 saturates the tanh form exactly in FP32, so its cubic is evaluated at
-// the clamped z and cannot overflow.
-__device__ __forceinline__ float act_sigmoid(float t) { return __fdividef(1.f, 1.f + __expf(-t)); }
-__device__ __forceinline__ float gelu_tanh_arg(float z) {   // 2 sqrt(2 / pi) (z + 0.044715 z^3)
-  const float c = fminf(fmaxf(z, -30.f), 30.f);
-  return c * fmaf(0.0713548162726f, c * c, 1.59576912160573f);
+// ---- activations, on pairs ------------------------------------------------------------------
+// exp2 and the reciprocal are the hardware's approximations (relative error about 2^-22.5 and
+// 2^-23, against the 2^-9 of the BF16 result).  Every form keeps its relative accuracy in the
+// tails, where 1 + tanh or 1 + erf would cancel, and passes NaN on.
+__device__ __forceinline__ float2 exp2_2(float2 v) {
+  float2 r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 rcp2(float2 v) {
+  float2 r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+constexpr float kLog2e = 1.44269504088896f;
+constexpr float kTanhA = 1.59576912160573f;      // 2 sqrt(2 / pi)
+constexpr float kTanhB = 0.0713548162726009f;    // 2 sqrt(2 / pi) 0.044715
+
+// 1 / (1 + exp(-w)) for w = k z (1 + ...): sigmoid of the SiLU's or the tanh GELU's argument.
+template <int kAct>
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+  float2 a;
+  if constexpr (kAct == kActSilu) {
+    a = mul2(z, both(-kLog2e));
+  } else {
+    a = mul2(z, fma2(mul2(z, z), both(-kLog2e * kTanhB), both(-kLog2e * kTanhA)));
+  }
+  return rcp2(add2(exp2_2(a), both(1.f)));
+}
+// Upper tail of the normal distribution at a = |z| (Q = erfc(a / sqrt 2) / 2) and exp(-a^2 / 2):
+// Q = exp(-a^2 / 2) t P(t) with t = 1 / (1 + 0.3 a), the form of Hastings' error function
+// approximations; P of degree 7 fitted here to the scaled complementary error function over
+// a <= 14 (relative error 1.5e-7; exp underflows beyond).
+__device__ __forceinline__ float2 normal_tail2(float2 a, float2& gauss) {
+  const float2 t = rcp2(fma2(a, both(0.3f), both(1.f)));
+  gauss = exp2_2(mul2(mul2(a, a), both(-0.5f * kLog2e)));
+  float2 q = both(0.03567494208754076f);
+  q = fma2(q, t, both(-0.15720365847955728f));
+  q = fma2(q, t, both(0.20635430300401225f));
+  q = fma2(q, t, both(-0.05368421566859173f));
+  q = fma2(q, t, both(0.12856185346333843f));
+  q = fma2(q, t, both(0.09991344303050201f));
+  q = fma2(q, t, both(0.12075396126465843f));
+  q = fma2(q, t, both(0.11962929862715543f));
+  return mul2(mul2(q, t), gauss);
 }
 
 template <int kAct>
-__device__ __forceinline__ float act_value(float z) {
-  if constexpr (kAct == kActRelu) return z > 0.f ? z : (z != z ? z : 0.f);
-  if constexpr (kAct == kActGelu) return 0.5f * z * erfcf(-0.707106781186548f * z);
-  if constexpr (kAct == kActGeluTanh) return z * act_sigmoid(gelu_tanh_arg(z));
-  if constexpr (kAct == kActSilu) return z * act_sigmoid(z);
+__device__ __forceinline__ float2 act_value2(float2 z) {
+  if constexpr (kAct == kActRelu) return make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f));
+  if constexpr (kAct == kActGelu) {
+    // z Phi(z) = max(z, 0) - |z| Q(|z|); |z| past 40 has Q = 0
+    const float2 a = make_float2(min_nan(fabsf(z.x), 40.f), min_nan(fabsf(z.y), 40.f));
+    float2 gauss;
+    const float2 q = normal_tail2(a, gauss);
+    return fma2(make_float2(-a.x, -a.y), q, make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f)));
+  }
+  if constexpr (kAct == kActGeluTanh || kAct == kActSilu) return mul2(z, sigmoid2<kAct>(z));
   return z;
 }
 
 // act(z) and act'(z)
 template <int kAct>
-__device__ __forceinline__ void act_value_slope(float z, float& value, float& slope) {
+__device__ __forceinline__ void act_value_slope2(float2 z, float2& value, float2& slope) {
   if constexpr (kAct == kActRelu) {
-    value = act_value<kActRelu>(z);
-    slope = z > 0.f ? 1.f : 0.f;
+    value = act_value2<kActRelu>(z);
+    slope = make_float2(z.x > 0.f ? 1.f : z.x <= 0.f ? 0.f : z.x, z.y > 0.f ? 1.f : z.y <= 0.f ? 0.f : z.y);
   } else if constexpr (kAct == kActGelu) {
-    const float phi = 0.5f * erfcf(-0.707106781186548f * z);
-    value = z * phi;
-    slope = fmaf(z * 0.398942280401433f, __expf(-0.5f * z * z), phi);
+    const float2 c = make_float2(max_nan(min_nan(z.x, 40.f), -40.f), max_nan(min_nan(z.y, 40.f), -40.f));
+    const float2 a = make_float2(fabsf(c.x), fabsf(c.y));
+    float2 gauss;
+    const float2 q = normal_tail2(a, gauss);
+    value = fma2(make_float2(-a.x, -a.y), q, make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f)));
+    const float2 phi = make_float2(z.x > 0.f ? 1.f - q.x : q.x, z.y > 0.f ? 1.f - q.y : q.y);
+    slope = fma2(mul2(c, both(0.398942280401433f)), gauss, phi);
   } else if constexpr (kAct == kActGeluTanh) {
-    const float c = fminf(fmaxf(z, -30.f), 30.f);
-    const float s = act_sigmoid(gelu_tanh_arg(z));
-    value = z * s;
-    slope = fmaf(c * s * (1.f - s), fmaf(0.214064448817800f, c * c, 1.59576912160573f), s);
+    // past |z| = 30 the sigmoid is 0 or 1 exactly, so its slope is taken at the clamped z, where
+    // the cubic does not overflow
+    const float2 c = make_float2(max_nan(min_nan(z.x, 30.f), -30.f), max_nan(min_nan(z.y, 30.f), -30.f));
+    const float2 s = sigmoid2<kAct>(c);
+    value = mul2(z, s);
+    const float2 rest = fma2(make_float2(-s.x, -s.y), s, s);                    // s (1 - s)
+    slope = fma2(mul2(c, rest), fma2(mul2(c, c), both(3.f * kTanhB), both(kTanhA)), s);
   } else if constexpr (kAct == kActSilu) {
-    const float s = act_sigmoid(z);
-    value = z * s;
-    slope = s * fmaf(z, 1.f - s, 1.f);
+    const float2 s = sigmoid2<kAct>(z);
+    value = mul2(z, s);
+    slope = mul2(s, fma2(z, add2(both(1.f), make_float2(-s.x, -s.y)), both(1.f)));
   } else {
     value = z;
-    slope = 1.f;
+    slope = both(1.f);
   }
 }
 
-// Runs f with the activation as a compile-time constant.
+// Runs f with the activation as a compile-time constant (the skinny schedule; the tiled schedules
+// are built once per activation: choosing among five inside them spilled 0.6 KB per thread).
 template <class F>
 __device__ __forceinline__ void with_activation(int act, F f) {
   switch (act) {
@@ -137,63 +218,111 @@ __device__ __forceinline__ float epilogue_bias(const EpilogueParams& e, int n) {
                      : __ldg(static_cast<const float*>(e.bias) + n);
 }
 
+__device__ __forceinline__ float2 bits2(const uint32_t* v) {
+  return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
+}
+__device__ __forceinline__ void set_bits2(uint32_t* v, float2 f) {
+  v[0] = __float_as_uint(f.x);
+  v[1] = __float_as_uint(f.y);
+}
+
+// A 16-byte load that stays where it is written: the compiler would otherwise raise a tile's bias
+// and residual loads together and spill the accumulators.
+__device__ __forceinline__ uint4 load16_here(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
 // z of 32 consecutive columns of a row, in place of the accumulators' bits.
 __device__ __forceinline__ void epilogue_z32(uint32_t (&v)[32], float alpha, const EpilogueParams& e,
                                              int col, int N) {
+  if (!e.bias) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(alpha * __uint_as_float(v[i]));
-  if (!e.bias) return;
+    for (int i = 0; i < 32; i += 2) set_bits2(v + i, mul2(bits2(v + i), both(alpha)));
+    return;
+  }
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    if (col + 8 * g >= N) break;
-    float b[8];
-    if (e.bias_bf16) {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.bias) + col + 8 * g));
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    float2 b[4];
+    if (col + 8 * g >= N) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        b[2 * i] = __uint_as_float(w[i] << 16);
-        b[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-      }
+      for (int i = 0; i < 4; ++i) b[i] = both(0.f);
+    } else if (e.bias_bf16) {
+      const uint4 q = load16_here(static_cast<const uint16_t*>(e.bias) + col + 8 * g);
+      b[0] = unpack2(q.x); b[1] = unpack2(q.y); b[2] = unpack2(q.z); b[3] = unpack2(q.w);
     } else {
-      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(e.bias) + col + 8 * g);
-      const float4 lo = __ldg(q), hi = __ldg(q + 1);
-      b[0] = lo.x; b[1] = lo.y; b[2] = lo.z; b[3] = lo.w;
-      b[4] = hi.x; b[5] = hi.y; b[6] = hi.z; b[7] = hi.w;
+      const float* q = static_cast<const float*>(e.bias) + col + 8 * g;
+      const uint4 lo = load16_here(q), hi = load16_here(q + 4);
+      b[0] = bits2(&lo.x); b[1] = bits2(&lo.z);
+      b[2] = bits2(&hi.x); b[3] = bits2(&hi.z);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[8 * g + i] = __float_as_uint(__uint_as_float(v[8 * g + i]) + b[i]);
+    for (int i = 0; i < 4; ++i)
+      set_bits2(v + 8 * g + 2 * i, fma2(bits2(v + 8 * g + 2 * i), both(alpha), b[i]));
   }
 }
 
 // u of those columns: 32 values, or 16 (in v[0..15]) when gated.
+template <int A>
 __device__ __forceinline__ void epilogue_act32(uint32_t (&v)[32], const EpilogueParams& e) {
-  with_activation(e.activation, [&](auto act) {
-    constexpr int A = decltype(act)::value;
-    if (e.gated) {
+  if (e.gated) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        v[i] = __float_as_uint(act_value<A>(__uint_as_float(v[2 * i])) * __uint_as_float(v[2 * i + 1]));
-    } else if constexpr (A != kActNone) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(act_value<A>(__uint_as_float(v[i])));
+    for (int i = 0; i < 16; i += 2) {
+      const float2 p0 = bits2(v + 2 * i), p1 = bits2(v + 2 * i + 2);      // (gate, up) twice
+      set_bits2(v + i, mul2(act_value2<A>(make_float2(p0.x, p1.x)), make_float2(p0.y, p1.y)));
     }
-  });
-}
-
-// Adds beta * residual to 8 consecutive columns of D's row (col, row inside D).
-__device__ __forceinline__ void epilogue_residual8(float (&f)[8], const EpilogueParams& e, int row, int col,
-                                                   int M) {
-  if (!e.residual || row >= M || col >= e.n_out) return;
-  const uint4 q = *reinterpret_cast<const uint4*>(e.residual + int64_t(row) * e.n_out + col);
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  } else if constexpr (A != kActNone) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = fmaf(e.beta, __uint_as_float(w[i] << 16), f[2 * i]);
-    f[2 * i + 1] = fmaf(e.beta, __uint_as_float(w[i] & 0xFFFF0000u), f[2 * i + 1]);
+    for (int i = 0; i < 32; i += 2) set_bits2(v + i, act_value2<A>(bits2(v + i)));
   }
 }
 
+// The residual of kCols consecutive columns of D's row (zeros outside D).
+template <int kCols>
+struct ResidualRow {
+  uint4 q[kCols / 8];
+  __device__ __forceinline__ void fetch(const EpilogueParams& e, int row, int col, int M) {
+    if (!e.residual) return;
+    const uint16_t* p = e.residual + int64_t(row) * e.n_out + col;
+    const int n = row < M ? e.n_out - col : 0;
+#pragma unroll
+    for (int c = 0; c < kCols / 8; ++c) {
+      q[c] = make_uint4(0, 0, 0, 0);
+      if (8 * c < n) q[c] = load16_here(p + 8 * c);
+    }
+  }
+};
+// Asks for a warp's share of a tile ahead of use, while the tile's products are made: the bias of
+// its 128 columns into L1, its rows of the residual (one per lane) into L2.
+__device__ __forceinline__ void epilogue_prefetch(const EpilogueParams& e, int row, int col, int M, int N,
+                                                  int lane) {
+  const int n = col + 4 * lane;
+  if (e.bias && n < N) {
+    const char* p = static_cast<const char*>(e.bias) + int64_t(n) * (e.bias_bf16 ? 2 : 4);
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
+  }
+  if (e.residual && row + lane < M && col < N) {
+    const int dcol = e.gated ? col / 2 : col, cols = min(e.gated ? 64 : 128, e.n_out - dcol);
+    ptx::bulk_prefetch_l2(e.residual + int64_t(row + lane) * e.n_out + dcol, uint32_t(cols) * 2);
+  }
+}
+// BF16 of 8 FP32 values (their bits), plus beta * residual where q is given.
+__device__ __forceinline__ uint4 epilogue_pack8(const uint32_t* v, const EpilogueParams& e, const uint4* q) {
+  float2 f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = bits2(v + 2 * i);
+  if (q && e.residual) {
+    const uint32_t w[4] = {q->x, q->y, q->z, q->w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = fma2(unpack2(w[i]), both(e.beta), f[i]);
+  }
+  return make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y), pack_bf16x2(f[2].x, f[2].y),
+                    pack_bf16x2(f[3].x, f[3].y));
+}
 // Fills the kernels' parameters; box_cols: columns of the schedule's store box (0: no map).
 inline cudaError_t make_epilogue(EpilogueParams* p, const blackhole_sm100_epilogue& e, int M, int N,
                                  int box_cols) {
@@ -230,59 +359,47 @@ __global__ void __launch_bounds__(256) epilogue_backward_kernel(const __grid_con
   const int row1 = min(p.M, row0 + p.rows_per_chunk);
   ptx::pdl_launch_dependents();
   ptx::pdl_wait_prior_grid();
-  float acc[8];
+  float2 acc[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+  for (int i = 0; i < 4; ++i) acc[i] = both(0.f);
   if (col < p.N) {
     for (int row = row0 + warp; row < row1; row += 8) {
       const int64_t at = int64_t(row) * p.N + col;
       const uint4 zq = *reinterpret_cast<const uint4*>(p.z + at);
-      const uint32_t zw[4] = {zq.x, zq.y, zq.z, zq.w};
-      float z[8], g[8], d[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        z[2 * i] = __uint_as_float(zw[i] << 16);
-        z[2 * i + 1] = __uint_as_float(zw[i] & 0xFFFF0000u);
-      }
+      const float2 z[4] = {unpack2(zq.x), unpack2(zq.y), unpack2(zq.z), unpack2(zq.w)};
+      float2 g[4];
       if (p.gated) {
-        const uint2 q = *reinterpret_cast<const uint2*>(p.d + at / 2);
-        const uint32_t w[2] = {q.x, q.y};
+        const uint2 dq = *reinterpret_cast<const uint2*>(p.d + at / 2);
+        const float2 d[2] = {unpack2(dq.x), unpack2(dq.y)};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          d[2 * i] = __uint_as_float(w[i] << 16);
-          d[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float value, slope;
-          act_value_slope<kAct>(z[2 * i], value, slope);
-          g[2 * i] = d[i] * z[2 * i + 1] * slope;
-          g[2 * i + 1] = d[i] * value;
+          float2 value, slope;
+          act_value_slope2<kAct>(make_float2(z[2 * i].x, z[2 * i + 1].x), value, slope);
+          const float2 dg = mul2(mul2(d[i], make_float2(z[2 * i].y, z[2 * i + 1].y)), slope);
+          const float2 du = mul2(d[i], value);
+          g[2 * i] = make_float2(dg.x, du.x);
+          g[2 * i + 1] = make_float2(dg.y, du.y);
         }
       } else {
-        const uint4 q = *reinterpret_cast<const uint4*>(p.d + at);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        const uint4 dq = *reinterpret_cast<const uint4*>(p.d + at);
+        const float2 d[4] = {unpack2(dq.x), unpack2(dq.y), unpack2(dq.z), unpack2(dq.w)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          d[2 * i] = __uint_as_float(w[i] << 16);
-          d[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float value, slope;
-          act_value_slope<kAct>(z[i], value, slope);
-          g[i] = d[i] * slope;
+          float2 value, slope;
+          act_value_slope2<kAct>(z[i], value, slope);
+          g[i] = mul2(d[i], slope);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += g[i];
-      *reinterpret_cast<uint4*>(p.dz + at) = make_uint4(pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]),
-                                                        pack_bf16x2(g[4], g[5]), pack_bf16x2(g[6], g[7]));
+      for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], g[i]);
+      *reinterpret_cast<uint4*>(p.dz + at) =
+          make_uint4(pack_bf16x2(g[0].x, g[0].y), pack_bf16x2(g[1].x, g[1].y), pack_bf16x2(g[2].x, g[2].y),
+                     pack_bf16x2(g[3].x, g[3].y));
     }
   }
   if (!p.dbias) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc_s[warp][lane * 8 + i] = acc[i];
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<float2*>(&acc_s[warp][lane * 8 + 2 * i]) = acc[i];
   __syncthreads();
   const int c = blockIdx.x * kEpilogueBackCols + threadIdx.x;
   float s = 0.f;

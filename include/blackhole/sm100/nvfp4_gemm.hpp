@@ -99,6 +99,28 @@ inline cudaError_t library_workspace(int dev, cudaStream_t stream, int64_t bytes
 
 }  // namespace detail
 
+namespace detail {
+
+// Runs f with the activation of `epi` (kNoEpilogue without one) as a compile-time constant.
+template <bool kFused, class F>
+inline cudaError_t dispatch_activation(const blackhole_sm100_epilogue* epi, F f) {
+  if constexpr (!kFused) {
+    return f(std::integral_constant<int, kNoEpilogue>{});
+  } else {
+    switch (epi->activation) {
+      case kActRelu: return f(std::integral_constant<int, kActRelu>{});
+      case kActGelu: return f(std::integral_constant<int, kActGelu>{});
+      case kActGeluTanh: return f(std::integral_constant<int, kActGeluTanh>{});
+      case kActSilu: return f(std::integral_constant<int, kActSilu>{});
+      default: return f(std::integral_constant<int, kActNone>{});
+    }
+  }
+}
+template <class KT, int kAct>
+using schedule_traits = std::conditional_t<kAct != kNoEpilogue, FusedTraits<KT>, KT>;
+
+}  // namespace detail
+
 // Full control: element format, schedule choice and (for the skinny schedule) a caller-owned
 // workspace.  workspace == nullptr selects the library-owned workspace.
 // kFused: the result goes through the epilogue `epi` (gemm_epilogue.hpp) on its way to D.
@@ -128,11 +150,17 @@ inline cudaError_t block_scaled_bf16_gemm_ex(int M, int N, int K, void const* A,
                           : Nvfp4Schedule::kTwoSm;
   switch (schedule) {
     case Nvfp4Schedule::kOneSm:
-      return detail::launch_1sm<Nvfp4GemmTraitsT<4, Fmt>, kFused>(M, N, K, A, SFA, B, SFB, D, alpha,
-                                                                   st, dev, stream, epi);
+      return detail::dispatch_activation<kFused>(epi, [&](auto act) {
+        constexpr int kAct = decltype(act)::value;
+        return detail::launch_1sm<detail::schedule_traits<Nvfp4GemmTraitsT<4, Fmt>, kAct>, kAct>(
+            M, N, K, A, SFA, B, SFB, D, alpha, st, dev, stream, epi);
+      });
     case Nvfp4Schedule::kTwoSm:
-      return detail::launch_2sm<Nvfp4Gemm2SmTraitsT<5, Fmt>, kFused>(
-          M, N, K, A, SFA, B, SFB, D, alpha, st, dev, stream, nullptr, epi);
+      return detail::dispatch_activation<kFused>(epi, [&](auto act) {
+        constexpr int kAct = decltype(act)::value;
+        return detail::launch_2sm<detail::schedule_traits<Nvfp4Gemm2SmTraitsT<5, Fmt>, kAct>, kAct>(
+            M, N, K, A, SFA, B, SFB, D, alpha, st, dev, stream, nullptr, epi);
+      });
     case Nvfp4Schedule::kSkinny:
     case Nvfp4Schedule::kSkinnyNoPrefetch: {
       if (M > 128) return cudaErrorInvalidValue;

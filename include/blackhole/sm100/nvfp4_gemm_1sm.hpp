@@ -56,6 +56,8 @@ struct Nvfp4GemmTraitsT {
 
   static constexpr int NumWarps = 10;
   static constexpr int NumThreads = NumWarps * 32;
+  static constexpr bool RegSplit = false;        // (FusedTraits)
+  static constexpr int MinRegs = 0;
   static constexpr int ProducerWarp = 0;
   static constexpr int MmaWarp = 1;
   static constexpr int FirstEpiWarp = 2;
@@ -127,11 +129,12 @@ __device__ __forceinline__ void tile_coords(int tile, const Nvfp4GemmParams& p, 
 
 }  // namespace detail
 
-template <class KT, bool kFused = false>
+template <class KT, int kAct = kNoEpilogue>
 __global__ void __launch_bounds__(KT::NumThreads, 1)
     nvfp4_gemm_kernel(const __grid_constant__
-                      std::conditional_t<kFused, Nvfp4GemmFusedParams, Nvfp4GemmParams> p) {
+                      std::conditional_t<kAct != kNoEpilogue, Nvfp4GemmFusedParams, Nvfp4GemmParams> p) {
 #if defined(BLACKHOLE_ARCH_SM100)
+  constexpr bool kFused = kAct != kNoEpilogue;
   using namespace ptx;
   constexpr int S = KT::Stages;
 
@@ -189,6 +192,8 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
   const uint32_t tmem = *tmem_slot;
   // the previous kernel in the stream must be complete before global memory is touched
   pdl_wait_prior_grid();
+  if constexpr (KT::RegSplit)
+    if (warp < KT::FirstEpiWarp) setmaxnreg_dec<KT::ControlRegs>();   // (the first warpgroup)
 
   if (warp == KT::ProducerWarp) {
     // ------------------------------ TMA producer ------------------------------------
@@ -332,7 +337,8 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
       detail::drain_wait(drain_bar, 0);
     }
     __syncwarp();
-  } else {
+  } else if (!KT::RegSplit || warp >= KT::FirstEpiWarp) {
+    if constexpr (KT::RegSplit) setmaxnreg_inc<KT::EpiRegs>();
     // ------------------------------ epilogue ----------------------------------------
     const int q = warp & 3;                                   // TMEM lane quadrant
     const int half = (warp - KT::FirstEpiWarp) >> 2;          // column half of the tile
@@ -341,6 +347,9 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
     for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x) {
       int m_blk, n_blk;
       detail::tile_coords<KT>(tile, p, m_blk, n_blk);
+      if constexpr (kFused)
+        detail::epilogue_prefetch(p.epi, m_blk * KT::TileM + 32 * q, n_blk * KT::TileN + 128 * half, p.M, p.N,
+                                  lane);
       if (!wait_bounded_warp(acc_full, acc_phase, abort_flag, p.status, kStatusEpilogueTimeout)) break;
       tc_fence_after();
       uint32_t v0[32], v1[32], v2[32], v3[32];
@@ -392,20 +401,14 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
         }
       };
       if constexpr (kFused) {
-        // One 32 x 16 box of bits[0..15] (FP32) to `map` at (row0, col), after adding the
-        // residual when `d`.
-        auto store_box = [&](uint32_t* bits, const CUtensorMap* map, int col, int cols, bool d) {
+        // One 32 x 16 box of bits[0..15] (FP32) to `map` at (row0, col), plus the residual q.
+        auto store_box = [&](const uint32_t* bits, const CUtensorMap* map, int col, int cols, const uint4* q) {
           if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float f[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(bits[8 * c + i]);
-            if (d) detail::epilogue_residual8(f, p.epi, row0 + lane, col + 8 * c, p.M);
-            st_shared_v4(my_row + ((c ^ sw) << 4), detail::pack_bf16x2(f[0], f[1]),
-                         detail::pack_bf16x2(f[2], f[3]), detail::pack_bf16x2(f[4], f[5]),
-                         detail::pack_bf16x2(f[6], f[7]));
+            const uint4 d = detail::epilogue_pack8(bits + 8 * c, p.epi, q ? q + c : nullptr);
+            st_shared_v4(my_row + ((c ^ sw) << 4), d.x, d.y, d.z, d.w);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -415,19 +418,17 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
           }
         };
         auto finish = [&](uint32_t (&v)[32], int c32) {
-          const int col = col0 + c32;
+          const int col = col0 + c32, dcol = p.epi.gated ? col / 2 : col;
           detail::epilogue_z32(v, a, p.epi, col, p.N);
+          detail::ResidualRow<32> res;           // (gated: its first half)
+          res.fetch(p.epi, row0 + lane, dcol, p.M);
           if (p.epi.has_z) {
-            store_box(v, &p.epi.tmap_z, col, p.N, false);
-            store_box(v + 16, &p.epi.tmap_z, col + 16, p.N, false);
+            store_box(v, &p.epi.tmap_z, col, p.N, nullptr);
+            store_box(v + 16, &p.epi.tmap_z, col + 16, p.N, nullptr);
           }
-          detail::epilogue_act32(v, p.epi);
-          if (p.epi.gated) {
-            store_box(v, &p.tmap_d, col / 2, p.epi.n_out, true);
-          } else {
-            store_box(v, &p.tmap_d, col, p.N, true);
-            store_box(v + 16, &p.tmap_d, col + 16, p.N, true);
-          }
+          detail::epilogue_act32<kAct>(v, p.epi);
+          store_box(v, &p.tmap_d, dcol, p.epi.n_out, res.q);
+          if (!p.epi.gated) store_box(v + 16, &p.tmap_d, dcol + 16, p.epi.n_out, res.q + 2);
         };
         finish(v0, 0);
         finish(v1, 32);
@@ -455,11 +456,12 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
 
 namespace detail {
 
-template <class KT, bool kFused = false>
+template <class KT, int kAct = kNoEpilogue>
 inline cudaError_t launch_1sm(int M, int N, int K, const void* A, const void* SFA, const void* B,
                               const void* SFB, void* D, float alpha, DeviceState* st, int dev,
                               cudaStream_t stream, const blackhole_sm100_epilogue* epi = nullptr) {
-  cudaError_t e = set_smem_once(nvfp4_gemm_kernel<KT, kFused>, KT::SmemBytes, dev);
+  constexpr bool kFused = kAct != kNoEpilogue;
+  cudaError_t e = set_smem_once(nvfp4_gemm_kernel<KT, kAct>, KT::SmemBytes, dev, KT::MinRegs);
   if (e != cudaSuccess) return e;
   std::conditional_t<kFused, Nvfp4GemmFusedParams, Nvfp4GemmParams> p;
   int n_out = N;
@@ -495,7 +497,7 @@ inline cudaError_t launch_1sm(int M, int N, int K, const void* A, const void* SF
     if (e != cudaSuccess) return e;
   }
   const int grid = p.num_tiles < st->num_sms ? p.num_tiles : st->num_sms;
-  e = launch_pdl(nvfp4_gemm_kernel<KT, kFused>, dim3(grid), dim3(KT::NumThreads), KT::SmemBytes, stream, p);
+  e = launch_pdl(nvfp4_gemm_kernel<KT, kAct>, dim3(grid), dim3(KT::NumThreads), KT::SmemBytes, stream, p);
   if (e != cudaSuccess) return e;
   return cudaGetLastError();
 }

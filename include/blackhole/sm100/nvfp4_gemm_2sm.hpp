@@ -87,6 +87,8 @@ struct Nvfp4Gemm2SmTraitsT {
   static constexpr int SfBufs = SfCopyWarp ? 4 : 1;
   static constexpr int NumWarps = SfCopyWarp ? 11 : 10;
   static constexpr int NumThreads = NumWarps * 32;
+  static constexpr bool RegSplit = false;        // (FusedTraits)
+  static constexpr int MinRegs = 0;
   static constexpr int ProducerWarp = 0;
   static constexpr int MmaWarp = 1;
   static constexpr int FirstEpiWarp = 2;
@@ -185,11 +187,12 @@ __device__ __forceinline__ void tile_coords_2sm(int tile, const Nvfp4Gemm2SmPara
 
 }  // namespace detail
 
-template <class KT, bool kGather = false, bool kFused = false>
+template <class KT, bool kGather = false, int kAct = kNoEpilogue>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
     nvfp4_gemm_2sm_kernel(const __grid_constant__
-                          std::conditional_t<kFused, Nvfp4Gemm2SmFusedParams, Nvfp4Gemm2SmParams> p) {
+                          std::conditional_t<kAct != kNoEpilogue, Nvfp4Gemm2SmFusedParams, Nvfp4Gemm2SmParams> p) {
 #if defined(BLACKHOLE_ARCH_SM100)
+  constexpr bool kFused = kAct != kNoEpilogue;
   using namespace ptx;
   constexpr int S = KT::Stages;
 
@@ -262,6 +265,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
   const uint32_t tmem = *tmem_slot;
   // the previous kernel in the stream must be complete before global memory is touched
   pdl_wait_prior_grid();
+  if constexpr (KT::RegSplit)
+    if (warp < KT::FirstEpiWarp) setmaxnreg_dec<KT::ControlRegs>();   // (the first warpgroup)
 
   if (warp == KT::ProducerWarp) {
     // ------------------------------ TMA producer (both CTAs) ------------------------
@@ -495,7 +500,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
       }
       __syncwarp();
     }
-  } else {
+  } else if (!KT::RegSplit || warp >= KT::FirstEpiWarp) {
+    if constexpr (KT::RegSplit) setmaxnreg_inc<KT::EpiRegs>();
     // ------------------------------ epilogue (both CTAs) ----------------------------
     const int q = warp & 3;
     const int half = (warp - KT::FirstEpiWarp) >> 2;
@@ -504,6 +510,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
     for (int tile = cluster; tile < p.num_tiles; tile += num_clusters) {
       int m_blk, n_blk;
       detail::tile_coords_2sm(tile, p, m_blk, n_blk);
+      if constexpr (kFused)
+        detail::epilogue_prefetch(p.epi, m_blk * KT::TileM + int(rank) * KT::CtaM + 32 * q,
+                                  n_blk * KT::TileN + 128 * half, p.M, p.N, lane);
       if (!wait_bounded_warp(acc_full, acc_phase, abort_flag, p.status, kStatusEpilogueTimeout)) break;
       tc_fence_after();
       uint32_t v0[32], v1[32], v2[32], v3[32];
@@ -609,20 +618,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
       };
       if constexpr (kFused) {
         // One 32 x 64 box to `map` at (row0, col): its 16-byte chunk c holds the FP32 bits
-        // chunk(c)[0..7], plus the residual when `d`.
-        auto store_box = [&](auto chunk, const CUtensorMap* map, int col, int cols, bool d) {
+        // chunk(c)[0..7], plus the residual q[c].
+        auto store_box = [&](auto chunk, const CUtensorMap* map, int col, int cols, const uint4* q) {
           if (lane == 0) bulk_wait_group_read<0>();   // previous box has been read out
           __syncwarp();
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            const uint32_t* bits = chunk(c);
-            float f[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(bits[i]);
-            if (d) detail::epilogue_residual8(f, p.epi, row0 + lane, col + 8 * c, p.M);
-            st_shared_v4(my_row + ((c ^ (lane & 7)) << 4), detail::pack_bf16x2(f[0], f[1]),
-                         detail::pack_bf16x2(f[2], f[3]), detail::pack_bf16x2(f[4], f[5]),
-                         detail::pack_bf16x2(f[6], f[7]));
+            const uint4 d = detail::epilogue_pack8(chunk(c), p.epi, q ? q + c : nullptr);
+            st_shared_v4(my_row + ((c ^ (lane & 7)) << 4), d.x, d.y, d.z, d.w);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -633,26 +636,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
         };
         auto chunk01 = [&](int c) -> const uint32_t* { return (c < 4 ? v0 : v1) + 8 * (c & 3); };
         auto chunk23 = [&](int c) -> const uint32_t* { return (c < 4 ? v2 : v3) + 8 * (c & 3); };
+        detail::ResidualRow<64> res;
         detail::epilogue_z32(v0, a, p.epi, col0, p.N);
         detail::epilogue_z32(v1, a, p.epi, col0 + 32, p.N);
+        if (p.epi.has_z) store_box(chunk01, &p.epi.tmap_z, col0, p.N, nullptr);
+        if (!p.epi.gated) res.fetch(p.epi, row0 + lane, col0, p.M);
+        detail::epilogue_act32<kAct>(v0, p.epi);
+        detail::epilogue_act32<kAct>(v1, p.epi);
+        if (!p.epi.gated) store_box(chunk01, &p.tmap_d, col0, p.N, res.q);
         detail::epilogue_z32(v2, a, p.epi, col0 + 64, p.N);
         detail::epilogue_z32(v3, a, p.epi, col0 + 96, p.N);
-        if (p.epi.has_z) {
-          store_box(chunk01, &p.epi.tmap_z, col0, p.N, false);
-          store_box(chunk23, &p.epi.tmap_z, col0 + 64, p.N, false);
-        }
-        detail::epilogue_act32(v0, p.epi);
-        detail::epilogue_act32(v1, p.epi);
-        detail::epilogue_act32(v2, p.epi);
-        detail::epilogue_act32(v3, p.epi);
+        if (p.epi.has_z) store_box(chunk23, &p.epi.tmap_z, col0 + 64, p.N, nullptr);
+        res.fetch(p.epi, row0 + lane, p.epi.gated ? col0 / 2 : col0 + 64, p.M);
+        detail::epilogue_act32<kAct>(v2, p.epi);
+        detail::epilogue_act32<kAct>(v3, p.epi);
         if (p.epi.gated) {
           auto pairs = [&](int c) -> const uint32_t* {
             return (c < 2 ? v0 : c < 4 ? v1 : c < 6 ? v2 : v3) + 8 * (c & 1);
           };
-          store_box(pairs, &p.tmap_d, col0 / 2, p.epi.n_out, true);
+          store_box(pairs, &p.tmap_d, col0 / 2, p.epi.n_out, res.q);
         } else {
-          store_box(chunk01, &p.tmap_d, col0, p.N, true);
-          store_box(chunk23, &p.tmap_d, col0 + 64, p.N, true);
+          store_box(chunk23, &p.tmap_d, col0 + 64, p.N, res.q);
         }
       } else {
         stage_store(v0, v1, 0);
@@ -675,7 +679,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
 
 namespace detail {
 
-template <class KT, bool kFused = false>
+template <class KT, int kAct = kNoEpilogue>
 inline cudaError_t launch_2sm(int M, int N, int K, const void* A, const void* SFA, const void* B,
                               const void* SFB, void* D, float alpha, DeviceState* st, int dev,
                               cudaStream_t stream, const GatherSpec* g = nullptr,
@@ -684,10 +688,11 @@ inline cudaError_t launch_2sm(int M, int N, int K, const void* A, const void* SF
   // the plain GEMM carries none of its code
   constexpr bool kCanGather = std::is_same_v<typename KT::Fmt, Nvfp4Format>;
   if (g && !kCanGather) return cudaErrorInvalidValue;
-  auto* kernel = nvfp4_gemm_2sm_kernel<KT, false, kFused>;
+  constexpr bool kFused = kAct != kNoEpilogue;
+  auto* kernel = nvfp4_gemm_2sm_kernel<KT, false, kAct>;
   if constexpr (kCanGather && !kFused)
     if (g) kernel = nvfp4_gemm_2sm_kernel<KT, true>;
-  cudaError_t e = set_smem_once(kernel, KT::SmemBytes, dev);
+  cudaError_t e = set_smem_once(kernel, KT::SmemBytes, dev, KT::MinRegs);
   if (e != cudaSuccess) return e;
   std::conditional_t<kFused, Nvfp4Gemm2SmFusedParams, Nvfp4Gemm2SmParams> p;
   int n_out = N;

@@ -384,17 +384,23 @@ inline DeviceState* prepare_device() {
   return &st;
 }
 
-// Sets a kernel's dynamic shared-memory limit once per (device, kernel function).
+// Sets a kernel's dynamic shared-memory limit once per (device, kernel function).  min_regs: the
+// registers per thread a kernel that splits its registers between warpgroups has to be launched
+// with; one compiled to fewer is refused (its split would never be granted).
 template <class Kernel>
-inline cudaError_t set_smem_once(Kernel kernel, int bytes, int dev) {
+inline cudaError_t set_smem_once(Kernel kernel, int bytes, int dev, int min_regs = 0) {
   static std::mutex mu;
   static std::map<std::pair<int, const void*>, cudaError_t> done;
   std::lock_guard<std::mutex> lock(mu);
   const auto key = std::make_pair(dev, reinterpret_cast<const void*>(kernel));
   auto it = done.find(key);
   if (it != done.end()) return it->second;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && min_regs > 0) {
+    cudaFuncAttributes a;
+    e = cudaFuncGetAttributes(&a, kernel);
+    if (e == cudaSuccess && a.numRegs < min_regs) e = cudaErrorInvalidDeviceFunction;
+  }
   done[key] = e;
   return e;
 }

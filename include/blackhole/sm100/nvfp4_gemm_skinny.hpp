@@ -508,6 +508,23 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
     Segment sg;
     while (w.next(sg)) {
       const bool finisher = sg.kt1 == p.kt_per_rb;
+      // the epilogue's own inputs are fetched before the sums are ready
+      [[maybe_unused]] float bias = 0.f;
+      [[maybe_unused]] uint16_t res[kFused ? EC : 1];
+      [[maybe_unused]] int nd = 0;
+      [[maybe_unused]] bool mine = false;
+      if constexpr (kFused) {
+        const int col = sg.rb * 128 + n_local;
+        nd = p.epi.gated ? col >> 1 : col;
+        mine = col < p.N && !(p.epi.gated && (col & 1));
+        if (finisher && col < p.N) {
+          bias = detail::epilogue_bias(p.epi, col);
+          if (p.epi.residual && mine)
+#pragma unroll
+            for (int m = 0; m < EC; ++m)
+              if (m0 + m < p.M) res[m] = p.epi.residual[int64_t(m0 + m) * p.epi.n_out + nd];
+        }
+      }
       float part[kEarlyPartials ? EC : 1];
       if constexpr (kEarlyPartials) {
 #pragma unroll
@@ -565,30 +582,34 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
         // lane above the up feature of the same column of D
         const detail::EpilogueParams& ep = p.epi;
         const bool in = n < p.N;
-        const float bias = in ? detail::epilogue_bias(ep, n) : 0.f;
 #pragma unroll
         for (int m = 0; m < EC; ++m) {
-          v[m] = fmaf(a, v[m], bias);
+          v[m] = ep.bias ? fmaf(a, v[m], bias) : a * v[m];
           if (ep.has_z && in && m0 + m < p.M)
             ep.z[int64_t(m0 + m) * p.N + n] = static_cast<uint16_t>(detail::pack_bf16x2(v[m], 0.f));
         }
         detail::with_activation(ep.activation, [&](auto act) {
           constexpr int A = decltype(act)::value;
 #pragma unroll
-          for (int m = 0; m < EC; ++m) {
-            const float up = ep.gated ? __shfl_xor_sync(0xFFFFFFFFu, v[m], 1) : 1.f;
-            v[m] = detail::act_value<A>(v[m]);
-            if (ep.gated) v[m] *= up;
+          for (int m = 0; m < EC; m += 2) {
+            if (m0 + m >= p.M) break;
+            float2 u = make_float2(v[m], v[m + 1]);
+            float2 up = u;
+            if (ep.gated) {
+              up.x = __shfl_xor_sync(0xFFFFFFFFu, u.x, 1);
+              up.y = __shfl_xor_sync(0xFFFFFFFFu, u.y, 1);
+            }
+            u = detail::act_value2<A>(u);
+            if (ep.gated) u = detail::mul2(u, up);
+            v[m] = u.x;
+            v[m + 1] = u.y;
           }
         });
-        const int nd = ep.gated ? n >> 1 : n;
-        const bool mine = in && !(ep.gated && (n & 1));
 #pragma unroll
         for (int m = 0; m < EC; ++m) {
           if (mine && m0 + m < p.M) {
-            const int64_t off = int64_t(m0 + m) * ep.n_out + nd;
-            if (ep.residual) v[m] = fmaf(ep.beta, detail::bf16_value(ep.residual[off]), v[m]);
-            p.d[off] = static_cast<uint16_t>(detail::pack_bf16x2(v[m], 0.f));
+            if (ep.residual) v[m] = fmaf(ep.beta, detail::bf16_value(res[m]), v[m]);
+            p.d[int64_t(m0 + m) * ep.n_out + nd] = static_cast<uint16_t>(detail::pack_bf16x2(v[m], 0.f));
           }
         }
       } else {

@@ -125,6 +125,19 @@ __device__ __forceinline__ bool wait_bounded_warp(uint32_t bar, uint32_t parity,
   }
 }
 
+// ---- register split between warpgroups ----------------------------------------------------
+// Every warp of a warpgroup executes the same one.  The shares of all warpgroups must fit what the
+// block was launched with (its registers per thread x threads), or the increase waits for good: the
+// launcher checks that (set_smem_once's min_regs).
+template <int N>
+__device__ __forceinline__ void setmaxnreg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void setmaxnreg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // ---- TMA / bulk copies -------------------------------------------------------------------
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
