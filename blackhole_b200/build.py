@@ -21,7 +21,6 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC,-fvisibility=hidden",
     "-Xptxas", "-v",
     "--expt-relaxed-constexpr",
-    "-split-compile=0",
     "-shared",
 ]
 

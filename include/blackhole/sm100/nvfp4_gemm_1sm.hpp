@@ -430,10 +430,16 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
           store_box(v, &p.tmap_d, dcol, p.epi.n_out, res.q);
           if (!p.epi.gated) store_box(v + 16, &p.tmap_d, dcol + 16, p.epi.n_out, res.q + 2);
         };
-        finish(v0, 0);
-        finish(v1, 32);
-        finish(v2, 64);
-        finish(v3, 96);
+#pragma unroll 1
+        for (int it = 0; it < 2; ++it) {       // (in a loop for the instruction cache's sake)
+          finish(v0, 64 * it);
+          finish(v1, 64 * it + 32);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            v0[i] = v2[i];
+            v1[i] = v3[i];
+          }
+        }
       } else {
         stage_store(v0, 0);
         stage_store(v1, 32);

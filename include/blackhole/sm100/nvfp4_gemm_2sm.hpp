@@ -510,7 +510,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
     for (int tile = cluster; tile < p.num_tiles; tile += num_clusters) {
       int m_blk, n_blk;
       detail::tile_coords_2sm(tile, p, m_blk, n_blk);
-      if constexpr (kFused)
+      if constexpr (kFused && !KT::SfCopyWarp)
         detail::epilogue_prefetch(p.epi, m_blk * KT::TileM + int(rank) * KT::CtaM + 32 * q,
                                   n_blk * KT::TileN + 128 * half, p.M, p.N, lane);
       if (!wait_bounded_warp(acc_full, acc_phase, abort_flag, p.status, kStatusEpilogueTimeout)) break;
@@ -617,16 +617,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
         }
       };
       if constexpr (kFused) {
-        // One 32 x 64 box to `map` at (row0, col): its 16-byte chunk c holds the FP32 bits
-        // chunk(c)[0..7], plus the residual q[c].
-        auto store_box = [&](auto chunk, const CUtensorMap* map, int col, int cols, const uint4* q) {
-          if (lane == 0) bulk_wait_group_read<0>();   // previous box has been read out
+        // 64 accumulator columns at a time, in a loop: unrolled over all 128 the epilogue's code
+        // pushed the MMA warp's loop out of the instruction cache.
+        auto box_free = [&]() {          // the previous box has been read out
+          if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const uint4 d = detail::epilogue_pack8(chunk(c), p.epi, q ? q + c : nullptr);
-            st_shared_v4(my_row + ((c ^ (lane & 7)) << 4), d.x, d.y, d.z, d.w);
-          }
+        };
+        auto put = [&](int c, const uint4& d) {      // 8 columns of this row
+          st_shared_v4(my_row + ((c ^ (lane & 7)) << 4), d.x, d.y, d.z, d.w);
+        };
+        auto box_store = [&](const CUtensorMap* map, int col, int cols) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && row0 < p.M && col < cols) {
@@ -634,29 +634,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
             bulk_commit_group();
           }
         };
-        auto chunk01 = [&](int c) -> const uint32_t* { return (c < 4 ? v0 : v1) + 8 * (c & 3); };
-        auto chunk23 = [&](int c) -> const uint32_t* { return (c < 4 ? v2 : v3) + 8 * (c & 3); };
-        detail::ResidualRow<64> res;
-        detail::epilogue_z32(v0, a, p.epi, col0, p.N);
-        detail::epilogue_z32(v1, a, p.epi, col0 + 32, p.N);
-        if (p.epi.has_z) store_box(chunk01, &p.epi.tmap_z, col0, p.N, nullptr);
-        if (!p.epi.gated) res.fetch(p.epi, row0 + lane, col0, p.M);
-        detail::epilogue_act32<kAct>(v0, p.epi);
-        detail::epilogue_act32<kAct>(v1, p.epi);
-        if (!p.epi.gated) store_box(chunk01, &p.tmap_d, col0, p.N, res.q);
-        detail::epilogue_z32(v2, a, p.epi, col0 + 64, p.N);
-        detail::epilogue_z32(v3, a, p.epi, col0 + 96, p.N);
-        if (p.epi.has_z) store_box(chunk23, &p.epi.tmap_z, col0 + 64, p.N, nullptr);
-        res.fetch(p.epi, row0 + lane, p.epi.gated ? col0 / 2 : col0 + 64, p.M);
-        detail::epilogue_act32<kAct>(v2, p.epi);
-        detail::epilogue_act32<kAct>(v3, p.epi);
-        if (p.epi.gated) {
-          auto pairs = [&](int c) -> const uint32_t* {
-            return (c < 2 ? v0 : c < 4 ? v1 : c < 6 ? v2 : v3) + 8 * (c & 1);
-          };
-          store_box(pairs, &p.tmap_d, col0 / 2, p.epi.n_out, res.q);
-        } else {
-          store_box(chunk23, &p.tmap_d, col0 + 64, p.N, res.q);
+        uint4 first[4];                  // gated: D's first 32 columns, kept for the second half's
+#pragma unroll 1
+        for (int it = 0; it < 2; ++it) {
+          const int col = col0 + 64 * it;
+          detail::epilogue_z32(v0, a, p.epi, col, p.N);
+          detail::epilogue_z32(v1, a, p.epi, col + 32, p.N);
+          if (p.epi.has_z) {
+            box_free();
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              put(c, detail::epilogue_pack8((c < 4 ? v0 : v1) + 8 * (c & 3), p.epi, nullptr));
+            box_store(&p.epi.tmap_z, col, p.N);
+          }
+          detail::ResidualRow<64> res;
+          res.fetch(p.epi, row0 + lane, p.epi.gated ? col / 2 : col, p.M);
+          detail::epilogue_act32<kAct>(v0, p.epi);
+          detail::epilogue_act32<kAct>(v1, p.epi);
+          if (p.epi.gated) {             // 32 columns of D, half a box
+            uint4 d[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              d[c] = detail::epilogue_pack8((c < 2 ? v0 : v1) + 8 * (c & 1), p.epi, res.q + c);
+            if (it == 1) {
+              box_free();
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                put(c, first[c]);
+                put(4 + c, d[c]);
+              }
+              box_store(&p.tmap_d, col0 / 2, p.epi.n_out);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) first[c] = d[c];
+          } else {
+            box_free();
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              put(c, detail::epilogue_pack8((c < 4 ? v0 : v1) + 8 * (c & 3), p.epi, res.q + c));
+            box_store(&p.tmap_d, col, p.N);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            v0[i] = v2[i];
+            v1[i] = v3[i];
+          }
         }
       } else {
         stage_store(v0, v1, 0);
