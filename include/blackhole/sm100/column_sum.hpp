@@ -28,8 +28,19 @@ __device__ __forceinline__ void column_sum_cta(const float* row0, const float* s
   float s = 0.f;
   if (col < cols) {
     if (row0 && ry == 0) s = row0[col];
-#pragma unroll 4
-    for (int64_t i = ry; i < count; i += 32) s += src[i * stride + col];
+    int64_t i = ry;
+    for (; i + 7 * 32 < count; i += 8 * 32) {       // eight loads in flight
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = src[(i + 32 * k) * stride + col];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = i + 32 * k < count ? src[(i + 32 * k) * stride + col] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += v[k];
   }
   smem[ry * 33 + cx] = s;
   __syncthreads();

@@ -360,6 +360,7 @@ template <int kAct>
 __global__ void __launch_bounds__(256) epilogue_backward_kernel(const __grid_constant__ EpilogueBackwardParams p) {
   __shared__ float acc_s[8][kEpilogueBackCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kRows = 4;
   const int col = blockIdx.x * kEpilogueBackCols + lane * 8;
   const int row0 = blockIdx.y * p.rows_per_chunk;
   const int row1 = min(p.M, row0 + p.rows_per_chunk);
@@ -369,38 +370,54 @@ __global__ void __launch_bounds__(256) epilogue_backward_kernel(const __grid_con
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i] = both(0.f);
   if (col < p.N) {
-    for (int row = row0 + warp; row < row1; row += 8) {
-      const int64_t at = int64_t(row) * p.N + col;
-      const uint4 zq = *reinterpret_cast<const uint4*>(p.z + at);
-      const float2 z[4] = {unpack2(zq.x), unpack2(zq.y), unpack2(zq.z), unpack2(zq.w)};
-      float2 g[4];
-      if (p.gated) {
-        const uint2 dq = *reinterpret_cast<const uint2*>(p.d + at / 2);
-        const float2 d[2] = {unpack2(dq.x), unpack2(dq.y)};
+    // kRows rows of a warp in flight together: with one the loads' latency set the pace
+    for (int row = row0 + warp; row < row1; row += 8 * kRows) {
+      uint4 zq[kRows], dq[kRows];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float2 value, slope;
-          act_value_slope2<kAct>(make_float2(z[2 * i].x, z[2 * i + 1].x), value, slope);
-          const float2 dg = mul2(mul2(d[i], make_float2(z[2 * i].y, z[2 * i + 1].y)), slope);
-          const float2 du = mul2(d[i], value);
-          g[2 * i] = make_float2(dg.x, du.x);
-          g[2 * i + 1] = make_float2(dg.y, du.y);
-        }
-      } else {
-        const uint4 dq = *reinterpret_cast<const uint4*>(p.d + at);
-        const float2 d[4] = {unpack2(dq.x), unpack2(dq.y), unpack2(dq.z), unpack2(dq.w)};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float2 value, slope;
-          act_value_slope2<kAct>(z[i], value, slope);
-          g[i] = mul2(d[i], slope);
+      for (int u = 0; u < kRows; ++u) {
+        const int64_t at = int64_t(row + 8 * u) * p.N + col;
+        zq[u] = dq[u] = make_uint4(0, 0, 0, 0);
+        if (row + 8 * u < row1) {
+          zq[u] = __ldcs(reinterpret_cast<const uint4*>(p.z + at));
+          if (p.gated) {
+            const uint2 q = __ldcs(reinterpret_cast<const uint2*>(p.d + at / 2));
+            dq[u].x = q.x;
+            dq[u].y = q.y;
+          } else {
+            dq[u] = __ldcs(reinterpret_cast<const uint4*>(p.d + at));
+          }
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], g[i]);
-      *reinterpret_cast<uint4*>(p.dz + at) =
-          make_uint4(pack_bf16x2(g[0].x, g[0].y), pack_bf16x2(g[1].x, g[1].y), pack_bf16x2(g[2].x, g[2].y),
-                     pack_bf16x2(g[3].x, g[3].y));
+      for (int u = 0; u < kRows; ++u) {
+        if (row + 8 * u >= row1) break;
+        const float2 z[4] = {unpack2(zq[u].x), unpack2(zq[u].y), unpack2(zq[u].z), unpack2(zq[u].w)};
+        const float2 d[4] = {unpack2(dq[u].x), unpack2(dq[u].y), unpack2(dq[u].z), unpack2(dq[u].w)};
+        float2 g[4];
+        if (p.gated) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float2 value, slope;
+            act_value_slope2<kAct>(make_float2(z[2 * i].x, z[2 * i + 1].x), value, slope);
+            const float2 dg = mul2(mul2(d[i], make_float2(z[2 * i].y, z[2 * i + 1].y)), slope);
+            const float2 du = mul2(d[i], value);
+            g[2 * i] = make_float2(dg.x, du.x);
+            g[2 * i + 1] = make_float2(dg.y, du.y);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float2 value, slope;
+            act_value_slope2<kAct>(z[i], value, slope);
+            g[i] = mul2(d[i], slope);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], g[i]);
+        *reinterpret_cast<uint4*>(p.dz + int64_t(row + 8 * u) * p.N + col) =
+            make_uint4(pack_bf16x2(g[0].x, g[0].y), pack_bf16x2(g[1].x, g[1].y), pack_bf16x2(g[2].x, g[2].y),
+                       pack_bf16x2(g[3].x, g[3].y));
+      }
     }
   }
   if (!p.dbias) return;
