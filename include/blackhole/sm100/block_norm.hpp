@@ -66,13 +66,12 @@ inline Geometry geometry(int H) {
 }
 
 // Row ranges: `teams` CTAs (or clusters), each of rows [row_begin(t), row_begin(t + 1)), as many
-// as are resident at once (148 SMs; 512 threads of 128 registers or 1024 of 64).  Fixed by the sizes
+// as are resident at once (512 threads of 128 registers per SM, 148 SMs).  Fixed by the sizes
 // alone, so the workspace size and the order of the column sums do not depend on the device.
-inline int row_teams(int rows, const Geometry& g, int threads_per_sm) {
-  const int per_sm = std::max(1, threads_per_sm / g.threads);
+inline int row_teams(int rows, const Geometry& g) {
+  const int per_sm = std::max(1, 512 / g.threads);
   return std::min(rows, std::max(1, 148 * per_sm / g.cluster));
 }
-constexpr int kBackwardThreadsPerSm = 512;
 BLACKHOLE_HD inline int64_t row_begin(int64_t team, int64_t rows, int64_t teams) {
   return team * rows / teams;
 }
@@ -81,13 +80,14 @@ BLACKHOLE_HD inline int64_t team_of(int64_t row, int64_t rows, int64_t teams) {
   return ((row + 1) * teams - 1) / rows;
 }
 
-// Ring of row stages in shared memory: as many as fit the CTA's share of the SM, 8 at most.
-constexpr int kRingBytesPerSm = 192 * 1024;       // vectors in registers
-constexpr int kRingBytesPerSmL1 = 128 * 1024;     // vectors from L1, which has the rest of the 256 KB
+// Shared memory of a CTA: its share of the SM's, for the ring of row stages (as many as fit, 8 at
+// most) and `vectors` FP32 values per column behind it.
+constexpr int kSharedBytes = 224 * 1024;
 constexpr int kMaxStages = 8;
-inline int ring_stages(const Geometry& g, int threads_per_sm, int stage_bytes, int rows_per_team) {
-  const int share = (threads_per_sm > 512 ? kRingBytesPerSmL1 : kRingBytesPerSm) /
-                    std::max(1, threads_per_sm / g.threads);
+inline int ring_stages(const Geometry& g, int stage_bytes, int vectors, int rows_per_team) {
+  const int per_sm = std::max(1, 512 / g.threads);
+  // (a CTA's static shared memory and its reservation besides, where several share an SM)
+  const int share = kSharedBytes / per_sm - (per_sm > 1 ? 2048 : 0) - vectors * 64 * g.threads;
   return std::max(1, std::min({share / stage_bytes, kMaxStages, rows_per_team}));
 }
 
@@ -95,7 +95,7 @@ inline int ring_stages(const Geometry& g, int threads_per_sm, int stage_bytes, i
 
 inline int64_t block_norm_backward_workspace_bytes(int rows, int H, int has_gate, int gate_rows) {
   if (rows < 1 || H < 8 || H > kNormMaxH || H % 8 != 0 || gate_rows < 0) return -1;
-  const int64_t teams = norm_detail::row_teams(rows, norm_detail::geometry(H), norm_detail::kBackwardThreadsPerSm);
+  const int64_t teams = norm_detail::row_teams(rows, norm_detail::geometry(H));
   const int64_t vectors = 4 + ((has_gate && gate_rows != 1) ? 2 : 0);
   return teams * vectors * H * 4;
 }
@@ -453,6 +453,28 @@ __device__ __forceinline__ void vector16(const void* p, int64_t at, int is_bf16,
   }
 }
 
+// FP32 vectors in shared memory of which every thread keeps and reads its own 16 values only, as
+// four 16-byte quarters a thread stride apart (no bank conflicts).
+struct OwnVectors {
+  uint8_t* base;
+  __device__ __forceinline__ float4* at(int k) const {
+    return reinterpret_cast<float4*>(base) + (k * 4) * blockDim.x + threadIdx.x;
+  }
+  __device__ __forceinline__ void put(int k, const Row16& v) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      at(k)[q * blockDim.x] = make_float4(v[2 * q].x, v[2 * q].y, v[2 * q + 1].x, v[2 * q + 1].y);
+  }
+  __device__ __forceinline__ void get(int k, Row16& v) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 t = at(k)[q * blockDim.x];
+      v[2 * q] = make_float2(t.x, t.y);
+      v[2 * q + 1] = make_float2(t.z, t.w);
+    }
+  }
+};
+
 // What a kernel is built for: RMS norms, RMS norms with a bias (or its gradient) somewhere, layer
 // norms.
 enum NormMode : int { kRms = 0, kRmsBias = 1, kLayerNorm = 2 };
@@ -554,14 +576,13 @@ __device__ __forceinline__ void quantize_row(const Row16& y, const Team& t, floa
 }
 
 // Forward.  kPost and p.o select what a row's p is made of; the gate row, the scale and the post
-// weight are one vector `cw`, made anew only where the gate row changes.  RMS norms keep their two
-// vectors in registers, one CTA of 512 threads per SM.  With biases there are four or five, and
-// layer norms wait longer for their sums: those kernels read the vectors again for every row
-// (from L1: their ring is smaller) and run with 64 registers, two CTAs per SM, so that one
-// computes while the other waits (layer norm at 9472 x 8192, FP32 stream, post norm: 270 us with
-// the vectors in registers).
+// weight are one vector `cw` (and with the post bias `cb`), made anew only where the gate row
+// changes.  RMS norms keep their two vectors in registers.  With biases there are up to four: those
+// kernels keep them as FP32 in shared memory, each thread its own columns (no barrier between),
+// behind a ring of fewer stages.  (In registers they spilled, and read from L1 for every row they
+// did not fit: layer norm of 9472 x 8192, FP32 stream, post norm, 270 and 259 us.)
 template <class TX, int kMode, bool kPost, int kCl>
-__global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, kMode == kRms ? 1 : 2)
+__global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
     block_norm_kernel(const __grid_constant__ NormParams p) {
 #if defined(BLACKHOLE_ARCH_SM100)
   constexpr bool kLayer = kMode == kLayerNorm, kBias = kMode != kRms;
@@ -588,7 +609,13 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, kMode == kRms
     for (int i = 0; i < p.stages && t.row0 + i < t.row1; ++i) fetch(t.row0 + i, i);
 
   Row16 w, cw;
-  if constexpr (!kBias) vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
+  OwnVectors own{ring + p.stages * stage_bytes};      // (kBias) 0: weight, 1: bias, 2: cw, 3: cb
+  vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
+  if constexpr (kBias) {
+    own.put(0, w);
+    vector16(p.bias, 0, p.param_bf16, t.col, t.live, 0.f, w);
+    own.put(1, w);
+  }
   const float quant_c = __frcp_rn(6.0f) * __frcp_rn(p.global_scale);    // quantize_kernel's estimate
   int gate_row = -1;
   const float inv_h = 1.0f / static_cast<float>(H);
@@ -597,20 +624,24 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, kMode == kRms
   for (int r = t.row0; r < t.row1; ++r) {
     const int64_t at = int64_t(r) * H;
     const int g = p.gate_rows ? r / p.gate_rows : 0;
-    if constexpr (!kBias) {
-      if (p.o && g != gate_row) {
-        gate_row = g;
-        vector16(p.gate, int64_t(g) * H, p.gate_bf16, t.col, t.live, p.scale, cw);
-        if (p.gate)
+    if (p.o && g != gate_row) {
+      gate_row = g;
+      vector16(p.gate, int64_t(g) * H, p.gate_bf16, t.col, t.live, 1.f, cw);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) cw[i] = mul2(cw[i], both(p.scale));
-        if constexpr (kPost) {
-          Row16 v;
-          vector16(p.post_weight, 0, p.param_bf16, t.col, t.live, 1.f, v);
+      for (int i = 0; i < 8; ++i) cw[i] = mul2(cw[i], both(p.scale));
+      if constexpr (kPost) {
+        Row16 v;
+        if constexpr (kBias) {
+          vector16(p.post_bias, 0, p.param_bf16, t.col, t.live, 0.f, v);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) cw[i] = mul2(cw[i], v[i]);
+          for (int i = 0; i < 8; ++i) v[i] = mul2(cw[i], v[i]);
+          own.put(3, v);
         }
+        vector16(p.post_weight, 0, p.param_bf16, t.col, t.live, 1.f, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) cw[i] = mul2(cw[i], v[i]);
       }
+      if constexpr (kBias) own.put(2, cw);
     }
     const uint32_t xs = t.ring + stage * stage_bytes;
     t.wait(stage, phase);
@@ -635,24 +666,18 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, kMode == kRms
           if constexpr (kLayer) o[i] = add2(o[i], both(-mean_post));
           o[i] = mul2(o[i], both(rstd_post));
         }
-        if constexpr (kBias) {
-          Row16 v;
-          vector16(p.post_weight, 0, p.param_bf16, t.col, t.live, 1.f, v);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = mul2(o[i], v[i]);
-          vector16(p.post_bias, 0, p.param_bf16, t.col, t.live, 0.f, v);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = add2(o[i], v[i]);
-        }
-      }
-      if constexpr (kBias) {
-        vector16(p.gate, int64_t(g) * H, p.gate_bf16, t.col, t.live, 1.f, cw);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = mul2(o[i], mul2(cw[i], both(p.scale)));
       }
       t.template read16<TX>(xs, h);
+      if constexpr (kBias) {
+        own.get(2, cw);
+        if constexpr (kPost) {
+          own.get(3, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = kBias ? add2(o[i], h[i]) : fma2(o[i], cw[i], h[i]);
+          for (int i = 0; i < 8; ++i) h[i] = add2(h[i], w[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = fma2(o[i], cw[i], h[i]);
       if (p.h) t.write16(static_cast<TX*>(p.h) + at, h);
     } else {
       t.template read16<TX>(xs, h);
@@ -677,14 +702,14 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, kMode == kRms
     if (p.stats && t.rank == 0 && tid == 0)
       reinterpret_cast<float4*>(p.stats)[r] = make_float4(mean_post, rstd_post, mean, rstd);
     if (p.out) {
-      if constexpr (kBias) vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
+      if constexpr (kBias) own.get(0, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if constexpr (kLayer) h[i] = add2(h[i], both(-mean));
         h[i] = mul2(mul2(h[i], both(rstd)), w[i]);
       }
       if constexpr (kBias) {
-        vector16(p.bias, 0, p.param_bf16, t.col, t.live, 0.f, w);
+        own.get(1, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[i] = add2(h[i], w[i]);
       }
@@ -968,18 +993,18 @@ static __global__ void __launch_bounds__(1024)
 }
 
 template <class P>
-inline cudaError_t launch_rows(void (*kernel)(P), P& p, const Geometry& g, int threads_per_sm, int stage_bytes,
+inline cudaError_t launch_rows(void (*kernel)(P), P& p, const Geometry& g, int stage_bytes, int vectors,
                                cudaStream_t s) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  e = detail::set_smem_once(kernel, kRingBytesPerSm, dev);
+  e = detail::set_smem_once(kernel, kSharedBytes, dev);
   if (e != cudaSuccess) return e;
   p.slice = g.slice;
-  p.teams = row_teams(p.rows, g, threads_per_sm);
-  p.stages = ring_stages(g, threads_per_sm, stage_bytes, (p.rows + p.teams - 1) / p.teams);
+  p.teams = row_teams(p.rows, g);
+  p.stages = ring_stages(g, stage_bytes, vectors, (p.rows + p.teams - 1) / p.teams);
   return detail::launch_pdl(kernel, dim3(p.teams * g.cluster), dim3(g.threads),
-                            static_cast<size_t>(p.stages) * stage_bytes, s, p);
+                            static_cast<size_t>(p.stages) * stage_bytes + size_t(vectors) * 64 * g.threads, s, p);
 }
 
 template <class TX, int kMode>
@@ -987,7 +1012,8 @@ inline cudaError_t launch_block_norm(NormParams& p, bool post, cudaStream_t s) {
   const Geometry g = geometry(p.H);
   auto* kernel = g.cluster == 1 ? (post ? block_norm_kernel<TX, kMode, true, 1> : block_norm_kernel<TX, kMode, false, 1>)
                                 : (post ? block_norm_kernel<TX, kMode, true, 2> : block_norm_kernel<TX, kMode, false, 2>);
-  return launch_rows(kernel, p, g, kMode == kRms ? 512 : 1024, 16 * g.threads * int(sizeof(TX) + (p.o ? 2 : 0)), s);
+  return launch_rows(kernel, p, g, 16 * g.threads * int(sizeof(TX) + (p.o ? 2 : 0)),
+                     kMode == kRms ? 0 : !p.o ? 2 : post ? 4 : 3, s);
 }
 
 template <class TX, int kMode, bool kPost, int kGate>
@@ -996,7 +1022,7 @@ inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, cudaStream_
   auto* kernel = g.cluster == 1 ? block_norm_backward_kernel<TX, kMode, kPost, kGate, 1>
                                 : block_norm_backward_kernel<TX, kMode, kPost, kGate, 2>;
   const int per = (p.dy ? int(sizeof(TX)) + 2 : 0) + (p.dh ? int(sizeof(TX)) : 0) + (p.o ? 2 : 0);
-  return launch_rows(kernel, p, g, kBackwardThreadsPerSm, 16 * g.threads * per, s);
+  return launch_rows(kernel, p, g, 16 * g.threads * per, 0, s);
 }
 template <class TX, int kMode, bool kPost>
 inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, int gate, cudaStream_t s) {
