@@ -29,20 +29,26 @@ _NORM = struct.Struct("@9i3f11P")               # blackhole_sm100_block_norm_arg
 _NORM_BACKWARD = struct.Struct("@8if17Pq")      # blackhole_sm100_block_norm_backward_args
 
 _torch = None
+_raw_stream = None
 
 
 def _device():
     """torch, and the current CUDA device (-1 without one: raw pointers can still be passed)."""
-    global _torch
+    global _torch, _raw_stream
     if _torch is None:
         import torch
         _torch = torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     return _torch.cuda.current_device() if _torch.cuda.is_initialized() or _torch.cuda.is_available() else -1
 
 
 def _handle(stream, device):
     if stream is None:
-        return _torch.cuda.current_stream(device).cuda_stream if device >= 0 else 0
+        if device < 0:
+            return 0
+        if _raw_stream is not None:       # the same handle without a Stream object (1.8 us less)
+            return _raw_stream(device)
+        return _torch.cuda.current_stream(device).cuda_stream
     if type(stream) is int:
         return stream
     if stream.device.index != device:

@@ -434,6 +434,14 @@ struct RowTeam {
     for (int k = 0; k < 2; ++k)
       if (live[k]) store8(row + col[k], v + 4 * k);
   }
+  // Asks for this thread's 16 values of a vector in L1.
+  __device__ __forceinline__ void prefetch16(const void* p, int64_t at, int is_bf16) const {
+    if (!p) return;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (live[k])
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p) + (at + col[k]) * (is_bf16 ? 2 : 4)));
+  }
   // Every thread of the CTA has read the stage.
   __device__ __forceinline__ void release_barrier() const { __syncthreads(); }
 };
@@ -792,6 +800,13 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
   if (tid == 0)
     for (int i = 0; i < p.stages && t.row0 + i < t.row1; ++i) fetch(t.row0 + i, i);
 
+  // the vectors that are read inside a row's chain of sums, into L1 meanwhile
+  if constexpr (kBias && kPost) {
+    t.prefetch16(p.weight, 0, p.param_bf16);
+    t.prefetch16(p.post_weight, 0, p.param_bf16);
+    t.prefetch16(p.post_bias, 0, p.param_bf16);
+    if (kGate) t.prefetch16(p.gate, int64_t(p.gate_rows ? t.row0 / p.gate_rows : 0) * H, p.gate_bf16);
+  }
   constexpr bool kKeep = !kBias || !kPost;    // else the sums leave no registers for the vectors
   const float2 zero = make_float2(0.f, 0.f);
   Row16 w, c;

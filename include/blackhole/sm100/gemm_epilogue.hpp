@@ -207,6 +207,7 @@ struct EpilogueParams {
   float beta;
   int activation, gated, bias_bf16, has_z;
   int n_out;                 // columns of D
+  int residual_wide;         // residual rows start on 32-byte boundaries
 };
 
 __device__ __forceinline__ float bf16_value(uint16_t bits) {
@@ -237,6 +238,14 @@ __device__ __forceinline__ uint4 load16_here(const void* p) {
   return v;
 }
 
+// 32 bytes in one request (32-byte aligned): whole sectors where each lane reads a row of its own.
+__device__ __forceinline__ void load32_here(const void* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+               : "l"(p)
+               : "memory");
+}
+
 // z of 32 consecutive columns of a row, in place of the accumulators' bits.
 __device__ __forceinline__ void epilogue_z32(uint32_t (&v)[32], float alpha, const EpilogueParams& e,
                                              int col, int N) {
@@ -245,24 +254,33 @@ __device__ __forceinline__ void epilogue_z32(uint32_t (&v)[32], float alpha, con
     for (int i = 0; i < 32; i += 2) set_bits2(v + i, mul2(bits2(v + i), both(alpha)));
     return;
   }
+  const int n = N - col;
+  if (e.bias_bf16) {
+    uint4 q[4];
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    float2 b[4];
-    if (col + 8 * g >= N) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = both(0.f);
-    } else if (e.bias_bf16) {
-      const uint4 q = load16_here(static_cast<const uint16_t*>(e.bias) + col + 8 * g);
-      b[0] = unpack2(q.x); b[1] = unpack2(q.y); b[2] = unpack2(q.z); b[3] = unpack2(q.w);
-    } else {
-      const float* q = static_cast<const float*>(e.bias) + col + 8 * g;
-      const uint4 lo = load16_here(q), hi = load16_here(q + 4);
-      b[0] = bits2(&lo.x); b[1] = bits2(&lo.z);
-      b[2] = bits2(&hi.x); b[3] = bits2(&hi.z);
+    for (int g = 0; g < 4; ++g) {
+      q[g] = make_uint4(0, 0, 0, 0);
+      if (8 * g < n) q[g] = load16_here(static_cast<const uint16_t*>(e.bias) + col + 8 * g);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      set_bits2(v + 8 * g + 2 * i, fma2(bits2(v + 8 * g + 2 * i), both(alpha), b[i]));
+    for (int g = 0; g < 4; ++g) {
+      const uint32_t w[4] = {q[g].x, q[g].y, q[g].z, q[g].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        set_bits2(v + 8 * g + 2 * i, fma2(bits2(v + 8 * g + 2 * i), both(alpha), unpack2(w[i])));
+    }
+  } else {
+    uint4 q[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      q[g] = make_uint4(0, 0, 0, 0);
+      if (4 * g < n) q[g] = load16_here(static_cast<const float*>(e.bias) + col + 4 * g);
+    }
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      set_bits2(v + 4 * g, fma2(bits2(v + 4 * g), both(alpha), bits2(&q[g].x)));
+      set_bits2(v + 4 * g + 2, fma2(bits2(v + 4 * g + 2), both(alpha), bits2(&q[g].z)));
+    }
   }
 }
 
@@ -289,6 +307,14 @@ struct ResidualRow {
     if (!e.residual) return;
     const uint16_t* p = e.residual + int64_t(row) * e.n_out + col;
     const int n = row < M ? e.n_out - col : 0;
+    if (e.residual_wide) {
+#pragma unroll
+      for (int c = 0; c < kCols / 8; c += 2) {
+        q[c] = q[c + 1] = make_uint4(0, 0, 0, 0);
+        if (8 * c < n) load32_here(p + 8 * c, q[c], q[c + 1]);
+      }
+      return;
+    }
 #pragma unroll
     for (int c = 0; c < kCols / 8; ++c) {
       q[c] = make_uint4(0, 0, 0, 0);
@@ -341,6 +367,7 @@ inline cudaError_t make_epilogue(EpilogueParams* p, const blackhole_sm100_epilog
   p->bias_bf16 = e.bias_is_bf16 != 0;
   p->has_z = e.Z != nullptr;
   p->n_out = e.gated ? N / 2 : N;
+  p->residual_wide = p->n_out % 16 == 0 && (reinterpret_cast<uintptr_t>(e.residual) & 31u) == 0;
   if (e.Z && box_cols > 0) return make_d_tmap(&p->tmap_z, e.Z, M, N, box_cols);
   return cudaSuccess;
 }
