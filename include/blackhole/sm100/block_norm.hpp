@@ -434,14 +434,6 @@ struct RowTeam {
     for (int k = 0; k < 2; ++k)
       if (live[k]) store8(row + col[k], v + 4 * k);
   }
-  // Asks for this thread's 16 values of a vector in L1.
-  __device__ __forceinline__ void prefetch16(const void* p, int64_t at, int is_bf16) const {
-    if (!p) return;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (live[k])
-        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p) + (at + col[k]) * (is_bf16 ? 2 : 4)));
-  }
   // Every thread of the CTA has read the stage.
   __device__ __forceinline__ void release_barrier() const { __syncthreads(); }
 };
@@ -800,14 +792,9 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
   if (tid == 0)
     for (int i = 0; i < p.stages && t.row0 + i < t.row1; ++i) fetch(t.row0 + i, i);
 
-  // the vectors that are read inside a row's chain of sums, into L1 meanwhile
-  if constexpr (kBias && kPost) {
-    t.prefetch16(p.weight, 0, p.param_bf16);
-    t.prefetch16(p.post_weight, 0, p.param_bf16);
-    t.prefetch16(p.post_bias, 0, p.param_bf16);
-    if (kGate) t.prefetch16(p.gate, int64_t(p.gate_rows ? t.row0 / p.gate_rows : 0) * H, p.gate_bf16);
-  }
-  constexpr bool kKeep = !kBias || !kPost;    // else the sums leave no registers for the vectors
+  // where biases' sums leave no registers for the vectors, they are kept in shared memory
+  constexpr bool kKeep = !kBias || !kPost;
+  OwnVectors own{ring + p.stages * stage_bytes};      // (!kKeep) 0: weight, 1: c
   const float2 zero = make_float2(0.f, 0.f);
   Row16 w, c;
   auto make_c = [&](int g, Row16& out) {
@@ -817,7 +804,8 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
 #pragma unroll
     for (int i = 0; i < 8; ++i) out[i] = mul2(out[i], kPost ? mul2(v[i], both(p.scale)) : both(p.scale));
   };
-  if constexpr (kKeep) vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
+  vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
+  if constexpr (!kKeep) own.put(0, w);
   Row16 dw, db, sa, sb, dwp, dbp;
 #pragma unroll
   for (int i = 0; i < 8; ++i) dw[i] = db[i] = sa[i] = sb[i] = dwp[i] = dbp[i] = zero;
@@ -842,11 +830,10 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
   for (int r = t.row0; r < t.row1; ++r) {
     const int64_t at = int64_t(r) * H;
     const int g = kGate == 2 ? r / p.gate_rows : 0;
-    if constexpr (kKeep) {
-      if (p.o && g != gate_row) {
-        gate_row = g;
-        make_c(g, c);
-      }
+    if (p.o && g != gate_row) {
+      gate_row = g;
+      make_c(g, c);
+      if constexpr (!kKeep) own.put(1, c);
     }
     const float4 st = reinterpret_cast<const float4*>(p.stats)[r];
     const uint32_t base = t.ring + stage * stage_bytes;
@@ -862,7 +849,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
       Row16 n, a;
       t.template read16<TX>(base, n);
       t.template read16<__nv_bfloat16>(base + at_dy, a);
-      if constexpr (!kKeep) vector16(p.weight, 0, p.param_bf16, t.col, t.live, 1.f, w);
+      if constexpr (!kKeep) own.get(0, w);
       float2 s = zero, sm = zero;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -889,7 +876,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
     Row16 n;
     if (p.o) {
       t.template read16<__nv_bfloat16>(base + at_o, n);
-      if constexpr (!kKeep) make_c(g, c);
+      if constexpr (!kKeep) own.get(1, c);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if constexpr (kPost && kLayer) n[i] = add2(n[i], both(-st.x));
@@ -980,7 +967,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
 // y - 3 is a team, and the group is the one that crosses into it if it is the first it crosses into.
 static __global__ void __launch_bounds__(1024)
     block_norm_sums_kernel(const __grid_constant__ NormBackwardParams p) {
-  __shared__ float smem[32 * 33];
+  __shared__ detail::ColumnSumShared smem;
   ptx::pdl_launch_dependents();
   ptx::pdl_wait_prior_grid();
   const int64_t vec = int64_t(p.teams) * p.H;
@@ -1037,7 +1024,7 @@ inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, cudaStream_
   auto* kernel = g.cluster == 1 ? block_norm_backward_kernel<TX, kMode, kPost, kGate, 1>
                                 : block_norm_backward_kernel<TX, kMode, kPost, kGate, 2>;
   const int per = (p.dy ? int(sizeof(TX)) + 2 : 0) + (p.dh ? int(sizeof(TX)) : 0) + (p.o ? 2 : 0);
-  return launch_rows(kernel, p, g, 16 * g.threads * per, 0, s);
+  return launch_rows(kernel, p, g, 16 * g.threads * per, kMode != kRms && kPost ? 2 : 0, s);
 }
 template <class TX, int kMode, bool kPost>
 inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, int gate, cudaStream_t s) {
@@ -1107,7 +1094,7 @@ inline cudaError_t block_norm_backward(const blackhole_sm100_block_norm_backward
   if (e != cudaSuccess) return e;
   const int edges = a.dgate && a.gate_rows != 1 && p.teams > 1 ? std::min(p.groups, p.teams - 1 + (p.groups <= p.teams)) : 0;
   if (a.dweight || a.dbias || a.dpost_weight || a.dpost_bias || edges) {
-    const dim3 grid((a.H + 31) / 32, 4 + edges);
+    const dim3 grid((a.H + detail::kColumnSumCols - 1) / detail::kColumnSumCols, 4 + edges);
     e = detail::launch_pdl(block_norm_sums_kernel, grid, dim3(1024), 0, stream, p);
     if (e != cudaSuccess) return e;
   }

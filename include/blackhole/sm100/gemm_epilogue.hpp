@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(256) epilogue_backward_kernel(const __grid_con
 
 static __global__ void __launch_bounds__(1024)
     epilogue_bias_sum_kernel(const __grid_constant__ EpilogueBackwardParams p) {
-  __shared__ float smem[32 * 33];
+  __shared__ ColumnSumShared smem;
   ptx::pdl_launch_dependents();
   ptx::pdl_wait_prior_grid();
   column_sum_cta(nullptr, p.ws, p.chunks, p.N, p.dbias, p.N, blockIdx.x, smem);
@@ -537,7 +537,8 @@ inline cudaError_t gemm_fused_backward(int M, int N, const void* dD, const void*
   e = detail::launch_pdl(kernel, grid, dim3(256), 0, stream, p);
   if (e != cudaSuccess) return e;
   if (dbias && p.chunks > 1) {
-    e = detail::launch_pdl(detail::epilogue_bias_sum_kernel, dim3((N + 31) / 32), dim3(1024), 0, stream, p);
+    e = detail::launch_pdl(detail::epilogue_bias_sum_kernel, dim3((N + detail::kColumnSumCols - 1) / detail::kColumnSumCols), dim3(1024), 0,
+                           stream, p);
     if (e != cudaSuccess) return e;
   }
   return cudaGetLastError();
