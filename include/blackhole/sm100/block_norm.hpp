@@ -501,62 +501,66 @@ struct NormParams {
   float scale, eps, global_scale;
 };
 
-// Quantises 8 consecutive columns of this thread's row into `out` (the row's codes); neighbouring
-// lanes hold the other columns of the 16- or 32-column block.  Every lane of the warp calls it
-// (`live` false: past the row's end, all zero).  Recipes and roundings are those of
-// nvfp4_quant.hpp.  Returns the block's scale factor code.
-template <int kFmt>
-__device__ __forceinline__ uint32_t quantize8(const float2* y, bool live, float g, float c, uint8_t* out, int col) {
+// Quantisation of a row's 16 columns of this thread, two 8-column vectors; neighbouring lanes hold
+// the other columns of a vector's 16- or 32-column block, and the codes of a word's four scale
+// factors are on 8 (NVFP4) or 16 (MX) neighbouring lanes.  Every lane of the warp takes part (past
+// the row's end all zero).  Recipes and roundings are those of nvfp4_quant.hpp.
+__device__ __forceinline__ float max_abs8(const float2* y) {
   float m = max_abs3(max_abs3(max_abs3(y[0].x, y[0].y, y[1].x), y[1].y, y[2].x), y[2].y, y[3].x);
-  m = max_abs3(m, y[3].y, 0.f);
-  m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-  float2 v[4];
-  if constexpr (kFmt == kOutNvfp4) {
-    uint32_t q = 0, code = 0;
-    if (live && m > 0.f) {
-      // as in quantize_kernel: estimates, and exact quotients only next to a rounding threshold
-      const float ys = m * c;
-      code = quant_detail::ue4m3_cvt(quant_detail::near_ue4m3_threshold(ys) ? (m / 6.0f) / g : ys);
-      const float s = quant_detail::ue4m3_value(code);
-      if (s != 0.f) {
-        const float scale = s * g;
-        const float rs = quant_detail::rcp_approx(scale);
-        bool near = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = mul2(y[i], both(rs));
-          near |= quant_detail::near_e2m1_threshold(v[i].x) || quant_detail::near_e2m1_threshold(v[i].y);
-        }
-        if (near) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = make_float2(y[i].x / scale, y[i].y / scale);
-        }
-        q = e2m1x8(v);
-      }
-    }
-    if (live) *reinterpret_cast<uint32_t*>(out + col / 2) = q;
-    return code;
-  } else {
-    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-    const int ebits = static_cast<int>(__float_as_uint(m) >> 23);
-    const int e = ebits == 0 ? -127 : max(-127, ebits - (kFmt == kOutMxfp8 ? 135 : 129));   // <= 126
-    const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = mul2(y[i], both(inv));
-    if constexpr (kFmt == kOutMxfp4) {
-      const uint32_t q = e2m1x8(v);
-      if (live) *reinterpret_cast<uint32_t*>(out + col / 2) = q;
-    } else {
-      const uint32_t lo = quant_detail::e4m3x2_satfinite(v[0].x, v[0].y) | (quant_detail::e4m3x2_satfinite(v[1].x, v[1].y) << 16);
-      const uint32_t hi = quant_detail::e4m3x2_satfinite(v[2].x, v[2].y) | (quant_detail::e4m3x2_satfinite(v[3].x, v[3].y) << 16);
-      if (live) *reinterpret_cast<uint2*>(out + col) = make_uint2(lo, hi);
-    }
-    return live ? static_cast<uint32_t>(e + 127) : 0u;
-  }
+  return max_abs3(m, y[3].y, 0.f);
 }
 
-// A row's 16 columns of this thread, quantised, and the words of their scale factors: four groups'
-// codes, on 8 (NVFP4) or 16 neighbouring lanes, make one word of the row.
+// NVFP4: the scale factor's code; writes the 8 codes.
+__device__ __forceinline__ uint32_t quantize8_nvfp4(const float2* y, float m, bool live, float g, float c,
+                                                    uint8_t* out, int col) {
+  uint32_t q = 0, code = 0;
+  if (live && m > 0.f) {
+    // as in quantize_kernel: estimates, and exact quotients only next to a rounding threshold
+    const float ys = m * c;
+    code = quant_detail::ue4m3_cvt(quant_detail::near_ue4m3_threshold(ys) ? (m / 6.0f) / g : ys);
+    const float s = quant_detail::ue4m3_value(code);
+    if (s != 0.f) {
+      const float scale = s * g;
+      const float rs = quant_detail::rcp_approx(scale);
+      float2 v[4];
+      bool near = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = mul2(y[i], both(rs));
+        near |= quant_detail::near_e2m1_threshold(v[i].x) || quant_detail::near_e2m1_threshold(v[i].y);
+      }
+      if (near) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = make_float2(y[i].x / scale, y[i].y / scale);
+      }
+      q = e2m1x8(v);
+    }
+  }
+  if (live) *reinterpret_cast<uint32_t*>(out + col / 2) = q;
+  return code;
+}
+
+// MX: the shared exponent comes from the block maximum's exponent bits; writes the 8 codes.
+template <int kFmt>
+__device__ __forceinline__ uint32_t quantize8_mx(const float2* y, uint32_t ebits, bool live, uint8_t* out,
+                                                 int col) {
+  // exponent floor(log2 amax) - emax, at least -127 (at most 126 here)
+  const int e = max(-127, static_cast<int>(ebits) - (kFmt == kOutMxfp8 ? 135 : 129));
+  const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  float2 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = mul2(y[i], both(inv));
+  if constexpr (kFmt == kOutMxfp4) {
+    const uint32_t q = e2m1x8(v);
+    if (live) *reinterpret_cast<uint32_t*>(out + col / 2) = q;
+  } else {
+    const uint32_t lo = quant_detail::e4m3x2_satfinite(v[0].x, v[0].y) | (quant_detail::e4m3x2_satfinite(v[1].x, v[1].y) << 16);
+    const uint32_t hi = quant_detail::e4m3x2_satfinite(v[2].x, v[2].y) | (quant_detail::e4m3x2_satfinite(v[3].x, v[3].y) << 16);
+    if (live) *reinterpret_cast<uint2*>(out + col) = make_uint2(lo, hi);
+  }
+  return live ? static_cast<uint32_t>(e + 127) : 0u;
+}
+
 template <int kFmt, class Team>
 __device__ __forceinline__ void quantize_row(const Row16& y, const Team& t, float g, float c, void* out,
                                              uint8_t* sf, int64_t r, int H) {
@@ -564,14 +568,32 @@ __device__ __forceinline__ void quantize_row(const Row16& y, const Team& t, floa
   const int lane = threadIdx.x & 31, ri = static_cast<int>(r);
   uint8_t* const row = static_cast<uint8_t*>(out) + (kFmt == kOutMxfp8 ? r * H : r * H / 2);
   uint8_t* const sf_row = sf + int64_t(ri >> 7) * ((H / kVec + 3) / 4) * 512 + (ri & 31) * 16 + ((ri >> 5) & 3) * 4;
+  uint32_t code[2];
+  if constexpr (kFmt == kOutNvfp4) {
 #pragma unroll
-  for (int v = 0; v < 2; ++v) {
-    const uint32_t code = quantize8<kFmt>(y + 4 * v, t.live[v], g, c, row, t.col[v]);
-    uint32_t word = (lane % kPer) == 0 ? code << (8 * ((lane / kPer) & 3)) : 0u;
-#pragma unroll
-    for (int k = kPer; k < kLanes; k <<= 1) word |= __shfl_xor_sync(0xFFFFFFFFu, word, k);
-    if ((lane % kLanes) == 0 && t.live[v])
-      *reinterpret_cast<uint32_t*>(sf_row + (t.col[v] / (4 * kVec)) * 512) = word;
+    for (int v = 0; v < 2; ++v) {
+      float m = max_abs8(y + 4 * v);
+      m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+      code[v] = quantize8_nvfp4(y + 4 * v, m, t.live[v], g, c, row, t.col[v]);
+    }
+  } else {
+    // both vectors' exponents as two 16-bit halves of one word through the shuffles
+    uint32_t e = (__float_as_uint(max_abs8(y)) >> 23) | (__float_as_uint(max_abs8(y + 4)) >> 23 << 16);
+    e = __vmaxu2(e, __shfl_xor_sync(0xFFFFFFFFu, e, 1));
+    e = __vmaxu2(e, __shfl_xor_sync(0xFFFFFFFFu, e, 2));
+    code[0] = quantize8_mx<kFmt>(y, e & 0xFFFFu, t.live[0], row, t.col[0]);
+    code[1] = quantize8_mx<kFmt>(y + 4, e >> 16, t.live[1], row, t.col[1]);
+  }
+  // bytes of four groups, kPer lanes apart, to the first lane of each kLanes: one byte pair per
+  // vector after the first exchange, both words after the second
+  const uint32_t own = code[0] | (code[1] << 16);
+  const uint32_t two = own | (__shfl_xor_sync(0xFFFFFFFFu, own, kPer) << 8);
+  const uint32_t four = __shfl_xor_sync(0xFFFFFFFFu, two, 2 * kPer);
+  if (lane % kLanes == 0) {
+    if (t.live[0])
+      *reinterpret_cast<uint32_t*>(sf_row + (t.col[0] / (4 * kVec)) * 512) = (two & 0xFFFFu) | (four << 16);
+    if (t.live[1])
+      *reinterpret_cast<uint32_t*>(sf_row + (t.col[1] / (4 * kVec)) * 512) = (two >> 16) | (four & 0xFFFF0000u);
   }
 }
 
