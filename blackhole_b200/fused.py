@@ -1,7 +1,12 @@
 """What stands between the accumulators of one block-scaled product of a transformer and the
 operand of the next: the products with bias, activation and residual in their epilogue, the
 gradient through that epilogue, and the norms before and after a block with its gate and residual
-scale, forward and backward, over the C ABI of include/blackhole_sm100.h.
+scale, forward and backward, over the C ABI of include/blackhole_sm100.h.  Together with the quantised products they are a block's MLP:
+
+    block_norm(.., out_format="mxfp8")            residual, norm, quantised operand
+    mxf8f4_bf16_gemm_fused(.., gated=True)        gate / up projection, gated activation
+    mxfp8_quantize(..)
+    mxf8f4_bf16_gemm_fused(.., residual=h)        down projection, residual
 
 Buffers are torch tensors (checked: CUDA tensors of the current device, contiguous, of the
 documented type and at least the documented size) or raw integer device pointers (taken as they
@@ -11,7 +16,7 @@ from __future__ import annotations
 
 import struct
 
-from . import SCHEDULES, BlackholeError, _ptr, load
+from . import SCHEDULES, BlackholeError, load
 
 __all__ = ["ACTIVATIONS", "nvfp4_bf16_gemm_fused", "mxfp4_bf16_gemm_fused", "mxf8f4_bf16_gemm_fused",
            "gemm_fused_backward", "gemm_fused_backward_workspace_bytes", "NORM_KINDS", "NORM_OUTPUTS", "block_norm", "block_norm_backward",
@@ -78,6 +83,21 @@ def _at(name, t, numel, dtype, device):
     raise ValueError(f"{name}: {t.numel()} elements, {numel} are needed")
 
 
+def _operand(name, t, nbytes, device):
+    """The address of a quantised operand or its scale factors: any type, at least `nbytes`."""
+    if t is None:
+        return 0
+    if type(t) is int:
+        return t
+    try:
+        size = t.numel() * t.element_size()
+    except AttributeError:
+        raise TypeError(f"{name}: cannot take a device pointer from {type(t)!r}") from None
+    if size < nbytes:
+        raise ValueError(f"{name}: {size} bytes, {nbytes} are needed")
+    return _at(name, t, 0, t.dtype, device)
+
+
 def _kind(told_bf16, *tensors):
     """The type of a call's tensors of one kind (the stream, the parameters, the gate): that of the
     first one given, BF16 or FP32; for raw pointers what the caller says."""
@@ -98,7 +118,7 @@ def _blocked_bytes(rows, H, vec):
     return -(-rows // 128) * -(-(H // vec) // 4) * 512
 
 
-def _gemm_fused(name, M, N, K, A, SFA, B, SFB, D, alpha, bias, activation, gated, residual, beta, Z,
+def _gemm_fused(fmt, M, N, K, A, SFA, B, SFB, D, alpha, bias, activation, gated, residual, beta, Z,
                 bias_is_bf16, schedule, workspace, workspace_bytes, stream):
     dev = _device()
     handle, bf16 = _handle(stream, dev), _torch.bfloat16
@@ -107,12 +127,15 @@ def _gemm_fused(name, M, N, K, A, SFA, B, SFB, D, alpha, bias, activation, gated
     epi = _EPILOGUE.pack(ACTIVATIONS[activation], 1 if gated else 0, t_bias is bf16, beta,
                          _at("bias", bias, N, t_bias, dev), _at("residual", residual, n, bf16, dev),
                          _at("Z", Z, M * N, bf16, dev))
-    if workspace is not None and hasattr(workspace, "numel") and not workspace_bytes:
+    if hasattr(workspace, "numel"):
         workspace_bytes = workspace.numel() * workspace.element_size()
-    rc = getattr(load(), name)(M, N, K, _ptr(A), _ptr(SFA), _ptr(B), _ptr(SFB),
-                               _at("D", D, n, bf16, dev), alpha, epi, SCHEDULES[schedule],
-                               _ptr(workspace) if workspace is not None else None,
-                               workspace_bytes, handle)
+    vec = 16 if fmt == "nvfp4" else 32
+    name = f"blackhole_sm100_{fmt}_bf16_gemm_fused"
+    rc = getattr(load(), name)(
+        M, N, K, _operand("A", A, M * K if fmt == "mxf8f4" else M * K // 2, dev),
+        _operand("SFA", SFA, _blocked_bytes(M, K, vec), dev), _operand("B", B, N * K // 2, dev),
+        _operand("SFB", SFB, _blocked_bytes(N, K, vec), dev), _at("D", D, n, bf16, dev), alpha, epi,
+        SCHEDULES[schedule], _operand("workspace", workspace, 0, dev), workspace_bytes, handle)
     if rc != 0:
         raise BlackholeError(name, rc)
 
@@ -132,7 +155,7 @@ def nvfp4_bf16_gemm_fused(M: int, N: int, K: int, A, SFA, B, SFB, D, alpha: floa
     weights is row 2j of B, up row j row 2j + 1 (N % 16 == 0).  bias: N values, BF16 or FP32
     (bias_is_bf16 only matters for a raw pointer); residual: BF16 of D's shape, may be D itself;
     Z: BF16 M x N, receives z for gemm_fused_backward."""
-    _gemm_fused("blackhole_sm100_nvfp4_bf16_gemm_fused", M, N, K, A, SFA, B, SFB, D, alpha, bias,
+    _gemm_fused("nvfp4", M, N, K, A, SFA, B, SFB, D, alpha, bias,
                 activation, gated, residual, beta, Z, bias_is_bf16, schedule, workspace,
                 workspace_bytes, stream)
 
@@ -143,7 +166,7 @@ def mxfp4_bf16_gemm_fused(M: int, N: int, K: int, A, SFA, B, SFB, D, alpha: floa
                           schedule: str = "auto", workspace=None, workspace_bytes: int = 0,
                           stream=None) -> None:
     """mxfp4_bf16_gemm with the epilogue of nvfp4_bf16_gemm_fused."""
-    _gemm_fused("blackhole_sm100_mxfp4_bf16_gemm_fused", M, N, K, A, SFA, B, SFB, D, alpha, bias,
+    _gemm_fused("mxfp4", M, N, K, A, SFA, B, SFB, D, alpha, bias,
                 activation, gated, residual, beta, Z, bias_is_bf16, schedule, workspace,
                 workspace_bytes, stream)
 
@@ -154,7 +177,7 @@ def mxf8f4_bf16_gemm_fused(M: int, N: int, K: int, A, SFA, B, SFB, D, alpha: flo
                            schedule: str = "auto", workspace=None, workspace_bytes: int = 0,
                            stream=None) -> None:
     """mxf8f4_bf16_gemm with the epilogue of nvfp4_bf16_gemm_fused."""
-    _gemm_fused("blackhole_sm100_mxf8f4_bf16_gemm_fused", M, N, K, A, SFA, B, SFB, D, alpha, bias,
+    _gemm_fused("mxf8f4", M, N, K, A, SFA, B, SFB, D, alpha, bias,
                 activation, gated, residual, beta, Z, bias_is_bf16, schedule, workspace,
                 workspace_bytes, stream)
 

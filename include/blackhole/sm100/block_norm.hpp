@@ -46,6 +46,7 @@
 namespace blackhole::sm100 {
 
 constexpr int kNormMaxH = 16384;
+constexpr int kNormMaxRows = 1 << 30;  // (32-bit row arithmetic)
 constexpr int kNormSliceH = 8192;     // columns one CTA works on: 512 threads x 16
 
 enum NormOut : int { kOutBf16 = 0, kOutF32 = 1, kOutNvfp4 = 2, kOutMxfp4 = 3, kOutMxfp8 = 4 };
@@ -94,14 +95,14 @@ inline int ring_stages(const Geometry& g, int stage_bytes, int vectors, int rows
 }  // namespace norm_detail
 
 inline int64_t block_norm_backward_workspace_bytes(int rows, int H, int has_gate, int gate_rows) {
-  if (rows < 1 || H < 8 || H > kNormMaxH || H % 8 != 0 || gate_rows < 0) return -1;
+  if (rows < 1 || rows > kNormMaxRows || H < 8 || H > kNormMaxH || H % 8 != 0 || gate_rows < 0) return -1;
   const int64_t teams = norm_detail::row_teams(rows, norm_detail::geometry(H));
   const int64_t vectors = 4 + ((has_gate && gate_rows != 1) ? 2 : 0);
   return teams * vectors * H * 4;
 }
 
 inline cudaError_t block_norm_check(const blackhole_sm100_block_norm_args& a) {
-  if (a.rows < 1 || a.H < 8 || a.H > kNormMaxH || a.H % 8 != 0) return cudaErrorInvalidValue;
+  if (a.rows < 1 || a.rows > kNormMaxRows || a.H < 8 || a.H > kNormMaxH || a.H % 8 != 0) return cudaErrorInvalidValue;
   if (a.kind < 0 || a.kind > 1 || a.gate_rows < 0) return cudaErrorInvalidValue;
   if (!(a.eps >= 0.0f) || !std::isfinite(a.eps) || !std::isfinite(a.scale))
     return cudaErrorInvalidValue;
@@ -132,7 +133,7 @@ inline cudaError_t block_norm_check(const blackhole_sm100_block_norm_args& a) {
 }
 
 inline cudaError_t block_norm_backward_check(const blackhole_sm100_block_norm_backward_args& a) {
-  if (a.rows < 1 || a.H < 8 || a.H > kNormMaxH || a.H % 8 != 0) return cudaErrorInvalidValue;
+  if (a.rows < 1 || a.rows > kNormMaxRows || a.H < 8 || a.H > kNormMaxH || a.H % 8 != 0) return cudaErrorInvalidValue;
   if (a.kind < 0 || a.kind > 1 || a.gate_rows < 0 || !std::isfinite(a.scale))
     return cudaErrorInvalidValue;
   if (!a.h || !a.stats || !a.dx || (!a.dy && !a.dh)) return cudaErrorInvalidValue;

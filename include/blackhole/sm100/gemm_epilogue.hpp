@@ -299,14 +299,15 @@ __device__ __forceinline__ void epilogue_act32(uint32_t (&v)[32], const Epilogue
   }
 }
 
-// The residual of kCols consecutive columns of D's row (zeros outside D).
+// The residual of up to kCols consecutive columns of D's row (zeros outside D): half of them when
+// gated, as D has half the columns of the accumulators.
 template <int kCols>
 struct ResidualRow {
   uint4 q[kCols / 8];
   __device__ __forceinline__ void fetch(const EpilogueParams& e, int row, int col, int M) {
     if (!e.residual) return;
     const uint16_t* p = e.residual + int64_t(row) * e.n_out + col;
-    const int n = row < M ? e.n_out - col : 0;
+    const int n = row < M ? min(e.n_out - col, e.gated ? kCols / 2 : kCols) : 0;
     if (e.residual_wide) {
 #pragma unroll
       for (int c = 0; c < kCols / 8; c += 2) {
@@ -470,6 +471,8 @@ static __global__ void __launch_bounds__(1024)
 
 #endif  // __CUDACC__
 
+constexpr int kEpilogueMaxRows = 1 << 30;     // (32-bit row arithmetic)
+
 // Row chunks of the backward kernel: about eight CTAs per SM (148 SMs), each of whole sets of 8
 // rows.  Fixed by the sizes, so the workspace and the order of the sums are too.
 inline void epilogue_backward_chunks(int M, int N, int* chunks, int* rows_per_chunk) {
@@ -483,7 +486,7 @@ inline void epilogue_backward_chunks(int M, int N, int* chunks, int* rows_per_ch
 }
 
 inline int64_t gemm_fused_backward_workspace_bytes(int M, int N) {
-  if (M < 1 || N < 8 || N % 8 != 0) return -1;
+  if (M < 1 || M > kEpilogueMaxRows || N < 8 || N % 8 != 0) return -1;
   int chunks, rows;
   epilogue_backward_chunks(M, N, &chunks, &rows);
   return chunks == 1 ? 0 : int64_t(chunks) * N * 4;
@@ -493,7 +496,8 @@ inline int64_t gemm_fused_backward_workspace_bytes(int M, int N) {
 inline cudaError_t gemm_fused_backward_check(int M, int N, const void* dD, const void* Z, const void* dZ,
                                              const float* dbias, int activation, int gated,
                                              const void* workspace, int64_t workspace_bytes) {
-  if (M < 1 || N < 8 || N % 8 != 0 || (gated && N % 16 != 0)) return cudaErrorInvalidValue;
+  if (M < 1 || M > kEpilogueMaxRows || N < 8 || N % 8 != 0 || (gated && N % 16 != 0))
+    return cudaErrorInvalidValue;
   if (activation < kActNone || activation > kActSilu) return cudaErrorInvalidValue;
   if (!dD || !Z || !dZ) return cudaErrorInvalidValue;
   auto mis = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };

@@ -263,7 +263,7 @@ BLACKHOLE_SM100_API int blackhole_sm100_mxf8f4_bf16_gemm_fused(
  *   workspace : blackhole_sm100_gemm_fused_backward_workspace_bytes(M, N) bytes for dbias's sums
  *               (NULL without dbias or where that is 0); contents do not matter; calls sharing one
  *               must be ordered, replays of captured graphs among them
- * M >= 1, N % 8 == 0 (gated 16), 16-byte aligned.  dbias is summed in an order fixed by M and N. */
+ * 1 <= M <= 2^30, N % 8 == 0 (gated 16), 16-byte aligned.  dbias is summed in an order fixed by M and N. */
 BLACKHOLE_SM100_API int blackhole_sm100_gemm_fused_backward(int M, int N, const void* dD, const void* Z,
                                                             void* dZ, float* dbias, int activation,
                                                             int gated, void* workspace,
@@ -289,7 +289,7 @@ BLACKHOLE_SM100_API int64_t blackhole_sm100_gemm_fused_backward_workspace_bytes(
  *            padding written 0); sf is NULL for formats 0 and 1
  *   stats  : NULL, or rows x 4 FP32: mean and 1 / sqrt(var + eps) of the post norm, then of the
  *            norm (0, and 0 for a post norm that is not there; the mean of an RMS norm is 0)
- * rows >= 1; H % 8 == 0 (NVFP4 % 16, MX % 32), 8 <= H <= 16384; contiguous, 16-byte aligned,
+ * 1 <= rows <= 2^30; H % 8 == 0 (NVFP4 % 16, MX % 32), 8 <= H <= 16384; contiguous, 16-byte aligned,
  * outputs not over inputs (h == x excepted).  Statistics and sums are FP32.  Errors:
  * cudaErrorInvalidValue for what breaks these rules, else the launch status.  Asynchronous and
  * stream-ordered, a programmatic dependent of the kernel before it like the products. */

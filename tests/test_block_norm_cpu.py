@@ -19,7 +19,7 @@ def forward(**over):
 
 
 @pytest.mark.parametrize("over", [
-    dict(rows=0), dict(rows=-1), dict(H=0), dict(H=12), dict(H=16392), dict(H=264), dict(gate_rows=-1),
+    dict(rows=0), dict(rows=-1), dict(rows=(1 << 30) + 1), dict(H=0), dict(H=12), dict(H=16392), dict(H=264), dict(gate_rows=-1),
     dict(eps=-1e-6), dict(eps=float("nan")), dict(eps=float("inf")), dict(scale=float("nan")),
     dict(scale=float("inf")), dict(x=None), dict(out=None, h=None, sf=None, weight=None, bias=None),
     dict(o=None), dict(post_norm=False), dict(out=None), dict(sf=None), dict(out_format="bf16"),
@@ -44,7 +44,7 @@ def backward(**over):
 
 
 @pytest.mark.parametrize("over", [
-    dict(rows=0), dict(H=12), dict(H=16392), dict(gate_rows=-1), dict(scale=float("nan")), dict(h=None),
+    dict(rows=0), dict(rows=(1 << 30) + 1), dict(H=12), dict(H=16392), dict(gate_rows=-1), dict(scale=float("nan")), dict(h=None),
     dict(stats=None), dict(dx=None), dict(dy=None, dh=None), dict(o=None), dict(do=None),
     dict(post_norm=False), dict(gate=None), dict(workspace_bytes=8), dict(dx=A), dict(dx=A + 3 * STEP),
     dict(dx=A + 4 * STEP + 16), dict(dx=A + 6 * STEP), dict(do=A + 6 * STEP), dict(do=A + 2 * STEP),
@@ -84,5 +84,26 @@ def test_workspace_size(rows, H, gate, gr):
     n = bh.block_norm_backward_workspace_bytes(rows, H, gate, gr)
     per = (6 if gate and gr != 1 else 4) * H * 4
     assert n % per == 0 and 1 <= n // per <= min(rows, 148 * 16)
-    for bad in ((0, H, gr), (rows, H + 4, gr), (rows, 16392, gr), (rows, H, -1)):
+    for bad in ((0, H, gr), ((1 << 30) + 1, H, gr), (rows, H + 4, gr), (rows, 16392, gr), (rows, H, -1)):
         assert bh.block_norm_backward_workspace_bytes(bad[0], bad[1], gate, bad[2]) < 0
+
+
+def test_structs_match_the_header(tmp_path):
+    """The packed arguments have the C structs' sizes and offsets."""
+    import os
+    import subprocess
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "blackhole_sm100.h"\n'
+                   "int main(void) {\n"
+                   'printf("%zu %zu %zu %zu %zu %zu\\n", sizeof(blackhole_sm100_epilogue),\n'
+                   " sizeof(blackhole_sm100_block_norm_args), sizeof(blackhole_sm100_block_norm_backward_args),\n"
+                   " offsetof(blackhole_sm100_epilogue, bias), offsetof(blackhole_sm100_block_norm_args, x),\n"
+                   " offsetof(blackhole_sm100_block_norm_backward_args, workspace_bytes));\n}\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    exe = tmp_path / "sizes"
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), "-I", os.path.join(cuda, "include"), str(src),
+                    "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [fused._EPILOGUE.size, fused._NORM.size, fused._NORM_BACKWARD.size, 16, 48,
+                   fused._NORM_BACKWARD.size - 8]

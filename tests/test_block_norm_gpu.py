@@ -268,3 +268,81 @@ def test_captured_and_replayed():
         assert torch.equal(q["out"], Q["out"]) and torch.equal(q["sf"], Q["sf"])
         for k in R:
             assert torch.equal(R[k], r[k]), k
+
+
+def test_offsets_past_32_bits():
+    """2^31 elements and more: the last rows equal the same rows in a call of their own."""
+    rows, H, tail = (1 << 18) + 3, 8192, 3
+    c = C.make(tail, H, "rms", "bf16", post=True, gate="one", seed=6)
+    x, o = (torch.zeros((rows, H), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    x[-tail:], o[-tail:] = c["x"], c["o"]
+    h, q = torch.empty_like(x), torch.empty((rows, H), dtype=torch.uint8, device="cuda")
+    sf = torch.empty(bh.mxfp4_sf_storage_bytes(rows, H), dtype=torch.uint8, device="cuda")
+    st = torch.empty((rows, 4), device="cuda")
+    kw = dict(weight=c["weight"], post_norm=True, post_weight=c["post_weight"], gate=c["gate"], scale=c["scale"],
+              eps=c["eps"])
+    bh.block_norm(rows, H, x, q, o=o, h=h, stats=st, sf=sf, out_format="mxfp8", **kw)
+    small = call({**c, "bias": None, "post_bias": None}, "mxfp8")
+    assert torch.equal(q[-tail:], small["out"]) and torch.equal(h[-tail:], small["h"])
+    assert torch.equal(sf[-small["sf"].numel():], small["sf"]) and not q[:-tail].any()
+    del q, sf
+    dx, do = x, o                                  # written over what the backward pass does not read
+    dy, dh = (torch.zeros((rows, H), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    dy[-tail:], dh[-tail:] = c["dy"], c["dh"]
+    o2 = torch.zeros_like(o)
+    o2[-tail:] = c["o"]
+    dw, dg = torch.empty(H, device="cuda"), torch.empty((1, H), device="cuda")
+    bh.block_norm_backward(rows, H, h, st, dx, dy=dy, dh=dh, o=o2, do=do, dweight=dw, dgate=dg, **kw)
+    ref = C.backward64({**c, "bias": None, "post_bias": None}, h[-tail:], st[-tail:], c["dy"], c["dh"])
+    C.close(dx[-tail:], ref["dx"], ref["mag_dx"])
+    C.close(do[-tail:], ref["do"], ref["mag_do"])
+    C.close(dw, ref["dweight"], ref["mag_dweight"], units=C.sum_units(rows))
+    C.close(dg, ref["dgate"], ref["mag_dgate"], units=C.sum_units(rows))
+
+
+def test_several_threads_and_streams():
+    """Three host threads, each with its own stream and sizes, forward and backward at once."""
+    import threading
+    cases = [C.make(r, h, k, "bf16", post=True, gate=g, seed=r)
+             for r, h, k, g in ((300, 1024, "rms", "one"), (77, 4104, "layer", 11), (900, 512, "rms", "each"))]
+    want = [both(c) for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        c, (f, h, r) = cases[i], want[i]
+        s = torch.cuda.Stream()
+        try:
+            with torch.cuda.stream(s):
+                for _ in range(5):
+                    F = call(c, "bf16")
+                    R = backward(c, F["h"], F["stats"], c["dy"], c["dh"])
+                    s.synchronize()
+                    if not torch.equal(F["out"], f["out"]) or any(
+                            r[k] is not None and not torch.equal(r[k], R[k]) for k in r):
+                        bad.append(i)
+        except Exception as e:          # an exception in a thread is a failure too
+            bad.append((i, repr(e)))
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad
+
+
+def test_tensors_that_do_not_fit():
+    c = C.make(4, 256, "rms", "bf16", gate="one")
+    ok = dict(weight=c["weight"], o=c["o"], gate=c["gate"])
+    out = torch.empty((4, 256), dtype=torch.bfloat16, device="cuda")
+    bh.block_norm(4, 256, c["x"], out, **ok)
+    for over in (dict(o=c["o"].float()), dict(o=c["o"][:3]), dict(weight=c["weight"][:128]), dict(weight=c["weight"].half()),
+                 dict(bias=torch.zeros(256, dtype=torch.bfloat16, device="cuda")), dict(h=c["x"].float()),
+                 dict(gate=c["gate"].cpu()), dict(gate=c["gate"], gate_rows=2), dict(stats=torch.empty(4, 3, device="cuda")),
+                 dict(o=torch.zeros((256, 4), dtype=torch.bfloat16, device="cuda").T)):
+        with pytest.raises(ValueError):
+            bh.block_norm(4, 256, c["x"], out, **{**ok, **over})
+    with pytest.raises(ValueError):
+        bh.block_norm(4, 256, c["x"], torch.empty((4, 256), dtype=torch.uint8, device="cuda"), out_format="mxfp8",
+                      sf=torch.empty(8, dtype=torch.uint8, device="cuda"), **ok)
+    with pytest.raises(bh.BlackholeError):       # a workspace that is too small
+        both(c, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))

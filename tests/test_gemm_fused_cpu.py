@@ -53,7 +53,7 @@ def test_names_and_null_epilogue():
 
 
 @pytest.mark.parametrize("over", [
-    dict(M=0), dict(M=-4), dict(N=0), dict(N=12), dict(N=264), dict(dD=None), dict(Z=None), dict(dZ=None),
+    dict(M=0), dict(M=-4), dict(M=(1 << 30) + 1), dict(N=0), dict(N=12), dict(N=264), dict(dD=None), dict(Z=None), dict(dZ=None),
     dict(dD=A + 8), dict(Z=A + S + 2), dict(dZ=A + 2 * S + 4), dict(dbias=A + 3 * S + 8), dict(dZ=A),
     dict(dZ=A + S + 16), dict(dZ=A + 16, gated=False), dict(workspace_bytes=4, M=100000),
     dict(workspace=A + 4 * S + 8),

@@ -85,6 +85,9 @@ def test_schedule_refusals_and_missing_workspace():
         C.call(c, D=c["D"].float())
     with pytest.raises(ValueError):
         C.call(c, D=c["D"][:8])
+    for k in ("A", "SFA", "B", "SFB"):
+        with pytest.raises(ValueError):
+            C.call({**c, k: c[k][:-1]})
 
 
 @pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
@@ -279,3 +282,62 @@ def test_an_mlp_block_forward_and_backward():
         NC.close(got, r[name], r["mag_" + name], what=name)
     for name, got in (("dweight", dw), ("dpost_weight", dwp), ("dgate", dg.view(1, H))):
         NC.close(got, r[name], r["mag_" + name], units=NC.sum_units(T), what=name)
+
+
+def test_offsets_past_32_bits():
+    """D, Z, residual and the gradient with more than 2^31 elements: the last rows equal the same rows
+    in calls of their own."""
+    M, N, K, tail = 65536 + 40, 32768, 256, 40
+    c = C.make("mxfp4", tail, N, K, "gelu", bias="f32", residual=True, z=True, seed=3)
+    C.call(c)
+    A = torch.zeros((M, K // 2), dtype=torch.uint8, device="cuda")
+    A[-tail:] = c["A"].view(tail, K // 2)
+    SFA = torch.full((bh.mxfp4_sf_storage_bytes(M, K),), 127, dtype=torch.uint8, device="cuda")
+    SFA[-c["SFA"].numel():] = c["SFA"]                  # (65536 rows are whole 128-row blocks)
+    D, Z, res = (torch.zeros((M, N), dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    res[-tail:] = c["residual"]
+    bh.mxfp4_bf16_gemm_fused(M, N, K, A, SFA, c["B"], c["SFB"], D, c["alpha"], bias=c["bias"], activation="gelu",
+                             residual=res, Z=Z)
+    torch.cuda.synchronize()
+    C.check(c)
+    c["D"], c["Z"] = D[-tail:], Z[-tail:]
+    C.check(c)
+    dD, dZ = D, res
+    dD[:-tail] = 0
+    db = torch.empty(N, device="cuda")
+    bh.gemm_fused_backward(M, N, dD, Z, dZ, dbias=db, activation="gelu")
+    small, db2 = torch.empty((tail, N), dtype=torch.bfloat16, device="cuda"), torch.empty(N, device="cuda")
+    bh.gemm_fused_backward(tail, N, dD[-tail:], Z[-tail:], small, dbias=db2, activation="gelu")
+    assert torch.equal(dZ[-tail:], small) and not dZ[:-tail].any()
+    mag = small.float().abs().sum(0)
+    assert ((db - db2).abs() <= 200 * C.U * mag + 1e-30).all()
+
+
+def test_several_threads_and_streams():
+    """Three host threads, each with its own stream, shape and schedule, at once."""
+    import threading
+    cases = []
+    for M, gated in ((8, True), (150, False), (520, True)):
+        cases.append(C.make("nvfp4", M, 1024, 1024, "silu", gated, "bf16", True, True, seed=M))
+        C.call(cases[-1])
+    torch.cuda.synchronize()
+    want = [c["D"].clone() for c in cases]
+    bad = []
+
+    def work(i):
+        c, s = cases[i], torch.cuda.Stream()
+        try:
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    D = torch.zeros_like(want[i])
+                    C.call(c, D=D)
+                    s.synchronize()
+                    if not torch.equal(D, want[i]):
+                        bad.append(i)
+        except Exception as e:
+            bad.append((i, repr(e)))
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad and bh.device_status(0) == 0
