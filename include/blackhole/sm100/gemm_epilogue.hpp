@@ -61,8 +61,10 @@ inline cudaError_t epilogue_check_args(int M, int N, const void* D,
 
 // Warp roles of the tiled schedules with an epilogue: 4 control warps (TMA, MMA, scale-factor
 // copies, one idle) and 8 epilogue warps, so that registers can be split by warpgroup: an epilogue
-// warp holds a row's 128 accumulators, the residual fetched ahead and the activation's temporaries,
-// which at an even split (168 each) spilled 0.4-1.1 KB per thread.
+// warp holds a row's 128 accumulators, 64 columns of the residual and the activation's temporaries,
+// which at an even split (168 each) spilled 0.4-1.1 KB per thread.  (Sixteen epilogue warps of 64
+// columns: 2048 x 8192 x 2048 with GELU, bias, residual and Z 65 -> 55 us, but 8192^3 without any
+// of them 212 -> 227 us, through their 64-byte store rows.)
 template <class Base>
 struct FusedTraits : Base {
   static constexpr bool RegSplit = true;
@@ -323,26 +325,6 @@ struct ResidualRow {
     }
   }
 };
-// Asks for a warp's share of a tile ahead of use, while the tile's products are made: the bias of
-// its 128 columns into L1, its rows of the residual (one per lane) into L2.  (Plain loads whose
-// value nobody waits for: bulk prefetches queue in the copy engine before the operand loads and
-// cost 9% of an 8192^3 product.)
-__device__ __forceinline__ void epilogue_prefetch(const EpilogueParams& e, int row, int col, int M, int N,
-                                                  int lane) {
-  const int n = col + 4 * lane;
-  if (e.bias && n < N) {
-    const char* p = static_cast<const char*>(e.bias) + int64_t(n) * (e.bias_bf16 ? 2 : 4);
-    asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
-  }
-  if (e.residual && row + lane < M && col < N) {
-    const int dcol = e.gated ? col / 2 : col;
-    const uint16_t* p = e.residual + int64_t(row + lane) * e.n_out + dcol;
-    uint32_t unused;
-    asm volatile("ld.global.L2::128B.u32 %0, [%1];" : "=r"(unused) : "l"(p));
-    if (!e.gated && dcol + 64 < e.n_out)
-      asm volatile("ld.global.L2::128B.u32 %0, [%1];" : "=r"(unused) : "l"(p + 64));
-  }
-}
 // BF16 of 8 FP32 values (their bits), plus beta * residual where q is given.
 __device__ __forceinline__ uint4 epilogue_pack8(const uint32_t* v, const EpilogueParams& e, const uint4* q) {
   float2 f[4];

@@ -347,9 +347,6 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
     for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x) {
       int m_blk, n_blk;
       detail::tile_coords<KT>(tile, p, m_blk, n_blk);
-      if constexpr (kFused)
-        detail::epilogue_prefetch(p.epi, m_blk * KT::TileM + 32 * q, n_blk * KT::TileN + 128 * half, p.M, p.N,
-                                  lane);
       if (!wait_bounded_warp(acc_full, acc_phase, abort_flag, p.status, kStatusEpilogueTimeout)) break;
       tc_fence_after();
       uint32_t v0[32], v1[32], v2[32], v3[32];
@@ -431,7 +428,7 @@ __global__ void __launch_bounds__(KT::NumThreads, 1)
           if (!p.epi.gated) store_box(v + 16, &p.tmap_d, dcol + 16, p.epi.n_out, res.q + 2);
         };
 #pragma unroll 1
-        for (int it = 0; it < 2; ++it) {       // (in a loop for the instruction cache's sake)
+        for (int it = 0; it < 2; ++it) {       // (in a loop: unrolled it spilled)
           finish(v0, 64 * it);
           finish(v1, 64 * it + 32);
 #pragma unroll

@@ -510,9 +510,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
     for (int tile = cluster; tile < p.num_tiles; tile += num_clusters) {
       int m_blk, n_blk;
       detail::tile_coords_2sm(tile, p, m_blk, n_blk);
-      if constexpr (kFused && !KT::SfCopyWarp)
-        detail::epilogue_prefetch(p.epi, m_blk * KT::TileM + int(rank) * KT::CtaM + 32 * q,
-                                  n_blk * KT::TileN + 128 * half, p.M, p.N, lane);
       if (!wait_bounded_warp(acc_full, acc_phase, abort_flag, p.status, kStatusEpilogueTimeout)) break;
       tc_fence_after();
       uint32_t v0[32], v1[32], v2[32], v3[32];
@@ -617,8 +614,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KT::NumThreads, 1)
         }
       };
       if constexpr (kFused) {
-        // 64 accumulator columns at a time, in a loop: unrolled over all 128 the epilogue's code
-        // pushed the MMA warp's loop out of the instruction cache.
+        // 64 accumulator columns at a time, in a loop: half the code of all 128 unrolled, at the
+        // same speed.
         auto box_free = [&]() {          // the previous box has been read out
           if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
