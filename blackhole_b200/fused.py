@@ -44,7 +44,8 @@ def _device():
         import torch
         _torch = torch
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return _torch.cuda.current_device() if _torch.cuda.is_initialized() or _torch.cuda.is_available() else -1
+    cuda = _torch.cuda
+    return cuda.current_device() if cuda.is_initialized() or cuda.is_available() else -1
 
 
 def _handle(stream, device):

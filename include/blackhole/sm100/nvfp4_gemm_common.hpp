@@ -408,19 +408,24 @@ inline cudaError_t set_smem_once(Kernel kernel, int bytes, int dev, int min_regs
 // Launches with programmatic stream serialization, so the kernel may start while the
 // previous kernel in the stream drains (the kernels call pdl_wait_prior_grid() before they
 // touch global memory).
+// cluster_y > 1: clusters of that many blocks along y.
 template <class Params>
 inline cudaError_t launch_pdl(void (*kernel)(Params), dim3 grid, dim3 block, size_t smem,
-                              cudaStream_t stream, const Params& p) {
+                              cudaStream_t stream, const Params& p, unsigned cluster_y = 1) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = cluster_y;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster_y > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 

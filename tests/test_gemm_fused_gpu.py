@@ -159,7 +159,7 @@ def epilogue_grads(M, N, act, gated, seed=0):
 
 @pytest.mark.parametrize("act", list(bh.ACTIVATIONS))
 @pytest.mark.parametrize("gated", [False, True])
-@pytest.mark.parametrize("M,N", [(1, 16), (7, 1008), (333, 256), (5000, 272)])
+@pytest.mark.parametrize("M,N", [(1, 16), (7, 1008), (333, 256), (1024, 528), (1025, 304), (5000, 272)])
 def test_gradient_through_the_epilogue(M, N, gated, act):
     Z, dD, ref, err = epilogue_grads(M, N, act, gated, M)
     dZ = torch.full((M, N), float("nan"), dtype=torch.bfloat16, device="cuda")
