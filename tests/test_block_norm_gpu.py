@@ -176,6 +176,46 @@ def test_gradients(rows, H, stream, post, gate, kind):
     check_backward(c, r, C.backward64(c, h, f["stats"], c["dy"], c["dh"]))
 
 
+@pytest.mark.parametrize("rows,H,stream,gate", [(40, 640, "bf16", "one"), (5, 12296, "f32", 2), (700, 96, "f32", "each")])
+def test_rms_norms_with_biases(rows, H, stream, gate):
+    """RMS norms with both biases, their gradients, and types that differ: parameters BF16, gate BF16
+    beside an FP32 stream."""
+    c = C.make(rows, H, "rms", stream, post=True, gate=gate, params="bf16", seed=H)
+    c["gate"] = c["gate"].to(torch.bfloat16)
+    check_forward(c, call(c, "f32"))
+    f = call(c, "bf16")
+    db, dpb = (torch.full((H,), float("nan"), device="cuda") for _ in range(2))
+    r = backward(c, f["h"], f["stats"], c["dy"], c["dh"], dbias=db, dpost_bias=dpb)
+    r.update(dbias=db, dpost_bias=dpb)
+    check_backward(c, r, C.backward64(c, f["h"], f["stats"], c["dy"], c["dh"]))
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("H,stream", [(16384, "f32"), (8200, "bf16")])
+def test_rows_wider_than_one_cta(H, stream, kind):
+    """Clusters of two CTAs over many rows, several rows per cluster."""
+    c = C.make(170, H, kind, stream, post=True, gate=60, seed=H)
+    check_forward(c, call(c, "bf16"))
+    f, h, r = both(c)
+    check_backward(c, r, C.backward64(c, h, f["stats"], c["dy"], c["dh"]))
+
+
+def test_statistics_alone_and_gradients_of_one_side():
+    """stats without out; no dy, a gate group crossing teams; no eps."""
+    c = C.make(500, 256, "layer", "bf16", post=True, gate=33, seed=12)
+    c["eps"] = 0.0
+    ref = C.forward64(c)
+    st = torch.empty((500, 4), device="cuda")
+    h = torch.empty_like(c["x"])
+    bh.block_norm(500, 256, c["x"], None, kind="layer", eps=0.0, o=c["o"], post_norm=True,
+                  post_weight=c["post_weight"], post_bias=c["post_bias"], gate=c["gate"], gate_rows=33,
+                  scale=c["scale"], h=h, stats=st)
+    full = call(c, "bf16")
+    assert torch.equal(st, full["stats"]) and torch.equal(h, full["h"])
+    C.close(h, ref["h"], ref["mag_h"])
+    check_backward(c, backward(c, h, st, None, c["dh"]), C.backward64(c, h, st, None, c["dh"]))
+
+
 @pytest.mark.parametrize("rows", [5000, 9473])
 @pytest.mark.parametrize("gate", ["one", 37, 700])
 def test_gradients_many_rows(rows, gate):
