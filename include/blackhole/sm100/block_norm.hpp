@@ -326,24 +326,19 @@ struct RowExchange {
       return;
     }
     put(mw, m2);
-    const float4 *mq = reinterpret_cast<const float4*>(slots[set][0]), *cq = reinterpret_cast<const float4*>(counts);
-    float2 t = make_float2(0.f, 0.f);
+    // one warp's values per lane, merged by butterflies (the same in every lane; half the
+    // shared-memory traffic of every thread reading them all)
+    const int at = threadIdx.x & (kWarps - 1);
+    const float m = slots[set][0][at], c = counts[at];
+    float t = c * m, q = slots[set][1][at];
 #pragma unroll
-    for (int i = 0; i < kWarps / 4; ++i) {
-      const float4 m = mq[i], c = cq[i];
-      t = fma2(make_float2(m.x, m.y), make_float2(c.x, c.y), t);
-      t = fma2(make_float2(m.z, m.w), make_float2(c.z, c.w), t);
-    }
-    mean = (t.x + t.y) * inv_h;
-    float2 q = make_float2(total(1), 0.f);
+    for (int o = 1; o < kWarps; o <<= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+    mean = t * inv_h;
+    const float d = m - mean;
+    q = fmaf(c * d, d, q);
 #pragma unroll
-    for (int i = 0; i < kWarps / 4; ++i) {
-      const float4 m = mq[i], c = cq[i];
-      const float2 d0 = add2(make_float2(m.x, m.y), both(-mean)), d1 = add2(make_float2(m.z, m.w), both(-mean));
-      q = fma2(mul2(d0, make_float2(c.x, c.y)), d0, q);
-      q = fma2(mul2(d1, make_float2(c.z, c.w)), d1, q);
-    }
-    squares = q.x + q.y;
+    for (int o = 1; o < kWarps; o <<= 1) q += __shfl_xor_sync(0xFFFFFFFFu, q, o);
+    squares = q;
     set ^= 1;
   }
 };
