@@ -70,12 +70,14 @@ inline Geometry geometry(int H) {
 }
 
 // Row ranges: `teams` CTAs (or clusters), each of rows [row_begin(t), row_begin(t + 1)), as many
-// as are resident at once (512 threads of 128 registers per SM, 148 SMs).  Fixed by the sizes
+// as are resident at once (512 threads of 128 registers or 640 of 96 per SM, 148 SMs).  Fixed by the sizes
 // alone, so the workspace size and the order of the column sums do not depend on the device.
-inline int row_teams(int rows, const Geometry& g) {
-  const int per_sm = std::max(1, 512 / g.threads);
+inline int row_teams(int rows, const Geometry& g, int threads_per_sm) {
+  const int per_sm = std::max(1, threads_per_sm / g.threads);
   return std::min(rows, std::max(1, 148 * per_sm / g.cluster));
 }
+constexpr int kBackwardThreadsPerSm = 512;
+inline int forward_threads_per_sm(const Geometry& g) { return g.threads <= 320 ? 640 : 512; }
 BLACKHOLE_HD inline int64_t row_begin(int64_t team, int64_t rows, int64_t teams) {
   return team * rows / teams;
 }
@@ -88,8 +90,9 @@ BLACKHOLE_HD inline int64_t team_of(int64_t row, int64_t rows, int64_t teams) {
 // most) and `vectors` FP32 values per column behind it.
 constexpr int kSharedBytes = 224 * 1024;
 constexpr int kMaxStages = 8;
-inline int ring_stages(const Geometry& g, int stage_bytes, int vectors, int rows_per_team) {
-  const int per_sm = std::max(1, 512 / g.threads);
+inline int ring_stages(const Geometry& g, int threads_per_sm, int stage_bytes, int vectors,
+                       int rows_per_team) {
+  const int per_sm = std::max(1, threads_per_sm / g.threads);
   // (a CTA's static shared memory and its reservation besides, where several share an SM)
   const int share = kSharedBytes / per_sm - (per_sm > 1 ? 2048 : 0) - vectors * 64 * g.threads;
   return std::max(1, std::min({share / stage_bytes, kMaxStages, rows_per_team}));
@@ -99,7 +102,7 @@ inline int ring_stages(const Geometry& g, int stage_bytes, int vectors, int rows
 
 inline int64_t block_norm_backward_workspace_bytes(int rows, int H, int has_gate, int gate_rows) {
   if (rows < 1 || rows > kNormMaxRows || H < 8 || H > kNormMaxH || H % 8 != 0 || gate_rows < 0) return -1;
-  const int64_t teams = norm_detail::row_teams(rows, norm_detail::geometry(H));
+  const int64_t teams = norm_detail::row_teams(rows, norm_detail::geometry(H), norm_detail::kBackwardThreadsPerSm);
   const int64_t vectors = 4 + ((has_gate && gate_rows != 1) ? 2 : 0);
   return teams * vectors * H * 4;
 }
@@ -602,8 +605,12 @@ __device__ __forceinline__ void quantize_row(const Row16& y, const Team& t, floa
 // kernels keep them as FP32 in shared memory, each thread its own columns (no barrier between),
 // behind a ring of fewer stages: layer norm of 9472 x 8192, FP32 stream, post norm, 241 us.  (In
 // registers they spilled, 270 us; from L1 for every row they did not fit, 259 us.)
-template <class TX, int kMode, bool kPost, int kCl>
-__global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(512, 1)
+//
+// kThreads: 512 for rows of more than 5120 columns, 128 registers; 320 for narrower ones, built for
+// 96 registers so that two CTAs of 320 threads share an SM (layer norm of 9472 x 5120, BF16 stream:
+// 95 -> LN2 us; one CTA's 10 warps left most issue slots empty).
+template <class TX, int kMode, bool kPost, int kCl, int kThreads>
+__global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThreads, kThreads == 320 ? 2 : 1)
     block_norm_kernel(const __grid_constant__ NormParams p) {
 #if defined(BLACKHOLE_ARCH_SM100)
   constexpr bool kLayer = kMode == kLayerNorm, kBias = kMode != kRms;
@@ -1016,16 +1023,16 @@ static __global__ void __launch_bounds__(1024)
 }
 
 template <class P>
-inline cudaError_t launch_rows(void (*kernel)(P), P& p, const Geometry& g, int stage_bytes, int vectors,
-                               cudaStream_t s) {
+inline cudaError_t launch_rows(void (*kernel)(P), P& p, const Geometry& g, int threads_per_sm,
+                               int stage_bytes, int vectors, cudaStream_t s) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   e = detail::set_smem_once(kernel, kSharedBytes, dev);
   if (e != cudaSuccess) return e;
   p.slice = g.slice;
-  p.teams = row_teams(p.rows, g);
-  p.stages = ring_stages(g, stage_bytes, vectors, (p.rows + p.teams - 1) / p.teams);
+  p.teams = row_teams(p.rows, g, threads_per_sm);
+  p.stages = ring_stages(g, threads_per_sm, stage_bytes, vectors, (p.rows + p.teams - 1) / p.teams);
   return detail::launch_pdl(kernel, dim3(p.teams * g.cluster), dim3(g.threads),
                             static_cast<size_t>(p.stages) * stage_bytes + size_t(vectors) * 64 * g.threads, s, p);
 }
@@ -1033,9 +1040,10 @@ inline cudaError_t launch_rows(void (*kernel)(P), P& p, const Geometry& g, int s
 template <class TX, int kMode>
 inline cudaError_t launch_block_norm(NormParams& p, bool post, cudaStream_t s) {
   const Geometry g = geometry(p.H);
-  auto* kernel = g.cluster == 1 ? (post ? block_norm_kernel<TX, kMode, true, 1> : block_norm_kernel<TX, kMode, false, 1>)
-                                : (post ? block_norm_kernel<TX, kMode, true, 2> : block_norm_kernel<TX, kMode, false, 2>);
-  return launch_rows(kernel, p, g, 16 * g.threads * int(sizeof(TX) + (p.o ? 2 : 0)),
+  auto* kernel = g.cluster == 2    ? (post ? block_norm_kernel<TX, kMode, true, 2, 512> : block_norm_kernel<TX, kMode, false, 2, 512>)
+                 : g.threads > 320 ? (post ? block_norm_kernel<TX, kMode, true, 1, 512> : block_norm_kernel<TX, kMode, false, 1, 512>)
+                                   : (post ? block_norm_kernel<TX, kMode, true, 1, 320> : block_norm_kernel<TX, kMode, false, 1, 320>);
+  return launch_rows(kernel, p, g, g.cluster == 2 ? 512 : forward_threads_per_sm(g), 16 * g.threads * int(sizeof(TX) + (p.o ? 2 : 0)),
                      kMode == kRms ? 0 : !p.o ? 2 : post ? 4 : 3, s);
 }
 
@@ -1045,7 +1053,7 @@ inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, cudaStream_
   auto* kernel = g.cluster == 1 ? block_norm_backward_kernel<TX, kMode, kPost, kGate, 1>
                                 : block_norm_backward_kernel<TX, kMode, kPost, kGate, 2>;
   const int per = (p.dy ? int(sizeof(TX)) + 2 : 0) + (p.dh ? int(sizeof(TX)) : 0) + (p.o ? 2 : 0);
-  return launch_rows(kernel, p, g, 16 * g.threads * per, kMode != kRms && kPost ? 2 : 0, s);
+  return launch_rows(kernel, p, g, kBackwardThreadsPerSm, 16 * g.threads * per, kMode != kRms && kPost ? 2 : 0, s);
 }
 template <class TX, int kMode, bool kPost>
 inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, int gate, cudaStream_t s) {
