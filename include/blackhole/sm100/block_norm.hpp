@@ -76,8 +76,8 @@ inline int row_teams(int rows, const Geometry& g, int threads_per_sm) {
   const int per_sm = std::max(1, threads_per_sm / g.threads);
   return std::min(rows, std::max(1, 148 * per_sm / g.cluster));
 }
-constexpr int kBackwardThreadsPerSm = 512;
-inline int forward_threads_per_sm(const Geometry& g) { return g.threads <= 320 ? 640 : 512; }
+constexpr int kThreadsPerSm = 512;
+constexpr int kNarrowThreads = 320, kNarrowThreadsPerSm = 640;
 BLACKHOLE_HD inline int64_t row_begin(int64_t team, int64_t rows, int64_t teams) {
   return team * rows / teams;
 }
@@ -94,7 +94,7 @@ inline int ring_stages(const Geometry& g, int threads_per_sm, int stage_bytes, i
                        int rows_per_team) {
   const int per_sm = std::max(1, threads_per_sm / g.threads);
   // (a CTA's static shared memory and its reservation besides, where several share an SM)
-  const int share = kSharedBytes / per_sm - (per_sm > 1 ? 2048 : 0) - vectors * 64 * g.threads;
+  const int share = kSharedBytes / per_sm - (per_sm > 1 ? 1792 : 0) - vectors * 64 * g.threads;
   return std::max(1, std::min({share / stage_bytes, kMaxStages, rows_per_team}));
 }
 
@@ -102,7 +102,7 @@ inline int ring_stages(const Geometry& g, int threads_per_sm, int stage_bytes, i
 
 inline int64_t block_norm_backward_workspace_bytes(int rows, int H, int has_gate, int gate_rows) {
   if (rows < 1 || rows > kNormMaxRows || H < 8 || H > kNormMaxH || H % 8 != 0 || gate_rows < 0) return -1;
-  const int64_t teams = norm_detail::row_teams(rows, norm_detail::geometry(H), norm_detail::kBackwardThreadsPerSm);
+  const int64_t teams = norm_detail::row_teams(rows, norm_detail::geometry(H), norm_detail::kThreadsPerSm);
   const int64_t vectors = 4 + ((has_gate && gate_rows != 1) ? 2 : 0);
   return teams * vectors * H * 4;
 }
@@ -499,6 +499,7 @@ struct NormParams {
   uint8_t* sf;
   float* stats;
   int rows, H, slice, teams, stages;
+  int keep_cw;          // gate, scale and post weight kept as one vector
   int gate_rows, param_bf16, gate_bf16, out_format;
   float scale, eps, global_scale;
 };
@@ -603,14 +604,14 @@ __device__ __forceinline__ void quantize_row(const Row16& y, const Team& t, floa
 // weight are one vector `cw` (and with the post bias `cb`), made anew only where the gate row
 // changes.  RMS norms keep their two vectors in registers.  With biases there are up to four: those
 // kernels keep them as FP32 in shared memory, each thread its own columns (no barrier between),
-// behind a ring of fewer stages: layer norm of 9472 x 8192, FP32 stream, post norm, 241 us.  (In
-// registers they spilled, 270 us; from L1 for every row they did not fit, 259 us.)
+// behind a ring of fewer stages: layer norm of 9472 x 8192, FP32 stream, post norm, 218 us.  (In
+// registers they spilled, 270 us; from L1 for every row they did not fit, 259 us, against 241 then.)
 //
-// kThreads: 512 for rows of more than 5120 columns, 128 registers; 320 for narrower ones, built for
-// 96 registers so that two CTAs of 320 threads share an SM (layer norm of 9472 x 5120, BF16 stream:
-// 95 -> LN2 us; one CTA's 10 warps left most issue slots empty).
+// kThreads: 512 (128 registers), or for rows of at most 5120 columns 320, built for 96 registers so
+// that two CTAs of 320 threads share an SM (layer norm of 9472 x 5120, BF16 stream:
+// 95 -> 71 us; one CTA's 10 warps left most issue slots empty).
 template <class TX, int kMode, bool kPost, int kCl, int kThreads>
-__global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThreads, kThreads == 320 ? 2 : 1)
+__global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThreads, kThreads == kNarrowThreads ? 2 : 1)
     block_norm_kernel(const __grid_constant__ NormParams p) {
 #if defined(BLACKHOLE_ARCH_SM100)
   constexpr bool kLayer = kMode == kLayerNorm, kBias = kMode != kRms;
@@ -652,7 +653,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThreads, kThreads
   for (int r = t.row0; r < t.row1; ++r) {
     const int64_t at = int64_t(r) * H;
     const int g = p.gate_rows ? r / p.gate_rows : 0;
-    if (p.o && g != gate_row) {
+    if (p.o && (!kBias || p.keep_cw) && g != gate_row) {
       gate_row = g;
       vector16(p.gate, int64_t(g) * H, p.gate_bf16, t.col, t.live, 1.f, cw);
 #pragma unroll
@@ -669,7 +670,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThreads, kThreads
 #pragma unroll
         for (int i = 0; i < 8; ++i) cw[i] = mul2(cw[i], v[i]);
       }
-      if constexpr (kBias) own.put(2, cw);
+      if (kBias && p.keep_cw) own.put(2, cw);
     }
     const uint32_t xs = t.ring + stage * stage_bytes;
     t.wait(stage, phase);
@@ -697,7 +698,13 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThreads, kThreads
       }
       t.template read16<TX>(xs, h);
       if constexpr (kBias) {
-        own.get(2, cw);
+        if (p.keep_cw) {
+          own.get(2, cw);
+        } else {                         // (no post norm: the gate row itself, from L1)
+          vector16(p.gate, int64_t(g) * H, p.gate_bf16, t.col, t.live, 1.f, cw);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) cw[i] = mul2(cw[i], both(p.scale));
+        }
         if constexpr (kPost) {
           own.get(3, w);
 #pragma unroll
@@ -1040,11 +1047,25 @@ inline cudaError_t launch_rows(void (*kernel)(P), P& p, const Geometry& g, int t
 template <class TX, int kMode>
 inline cudaError_t launch_block_norm(NormParams& p, bool post, cudaStream_t s) {
   const Geometry g = geometry(p.H);
-  auto* kernel = g.cluster == 2    ? (post ? block_norm_kernel<TX, kMode, true, 2, 512> : block_norm_kernel<TX, kMode, false, 2, 512>)
-                 : g.threads > 320 ? (post ? block_norm_kernel<TX, kMode, true, 1, 512> : block_norm_kernel<TX, kMode, false, 1, 512>)
-                                   : (post ? block_norm_kernel<TX, kMode, true, 1, 320> : block_norm_kernel<TX, kMode, false, 1, 320>);
-  return launch_rows(kernel, p, g, g.cluster == 2 ? 512 : forward_threads_per_sm(g), 16 * g.threads * int(sizeof(TX) + (p.o ? 2 : 0)),
-                     kMode == kRms ? 0 : !p.o ? 2 : post ? 4 : 3, s);
+  const int stage_bytes = 16 * g.threads * int(sizeof(TX) + (p.o ? 2 : 0));
+  // FP32 vectors kept in shared memory: weight, bias, cw, cb.  Without a post norm cw is only the
+  // scaled gate row and may be left to L1.
+  int vectors = kMode == kRms ? 0 : !p.o ? 2 : post ? 4 : 3;
+  // the narrow build where its smaller share of shared memory still holds two rows
+  const int teams = row_teams(p.rows, g, kNarrowThreadsPerSm);
+  auto fits = [&](int v) {
+    return p.rows <= teams || ring_stages(g, kNarrowThreadsPerSm, stage_bytes, v, 2) == 2;
+  };
+  bool narrow = g.cluster == 1 && g.threads <= kNarrowThreads;
+  if (narrow && !fits(vectors)) {
+    narrow = vectors == 3 && fits(2);
+    if (narrow) vectors = 2;
+  }
+  p.keep_cw = kMode != kRms && vectors >= 3;
+  auto* kernel = narrow ? (post ? block_norm_kernel<TX, kMode, true, 1, kNarrowThreads> : block_norm_kernel<TX, kMode, false, 1, kNarrowThreads>)
+                 : g.cluster == 1 ? (post ? block_norm_kernel<TX, kMode, true, 1, 512> : block_norm_kernel<TX, kMode, false, 1, 512>)
+                                  : (post ? block_norm_kernel<TX, kMode, true, 2, 512> : block_norm_kernel<TX, kMode, false, 2, 512>);
+  return launch_rows(kernel, p, g, narrow ? kNarrowThreadsPerSm : kThreadsPerSm, stage_bytes, vectors, s);
 }
 
 template <class TX, int kMode, bool kPost, int kGate>
@@ -1053,7 +1074,7 @@ inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, cudaStream_
   auto* kernel = g.cluster == 1 ? block_norm_backward_kernel<TX, kMode, kPost, kGate, 1>
                                 : block_norm_backward_kernel<TX, kMode, kPost, kGate, 2>;
   const int per = (p.dy ? int(sizeof(TX)) + 2 : 0) + (p.dh ? int(sizeof(TX)) : 0) + (p.o ? 2 : 0);
-  return launch_rows(kernel, p, g, kBackwardThreadsPerSm, 16 * g.threads * per, kMode != kRms && kPost ? 2 : 0, s);
+  return launch_rows(kernel, p, g, kThreadsPerSm, 16 * g.threads * per, kMode != kRms && kPost ? 2 : 0, s);
 }
 template <class TX, int kMode, bool kPost>
 inline cudaError_t launch_block_norm_backward(NormBackwardParams& p, int gate, cudaStream_t s) {
