@@ -121,7 +121,7 @@ def _blocked_bytes(rows, H, vec):
 
 def _gemm_fused(fmt, M, N, K, A, SFA, B, SFB, D, alpha, bias, activation, gated, residual, beta, Z,
                 bias_is_bf16, schedule, workspace, workspace_bytes, stream):
-    dev = _device()
+    M, N, K, dev = int(M), int(N), int(K), _device()
     handle, bf16 = _handle(stream, dev), _torch.bfloat16
     n = M * (N // 2 if gated else N)
     t_bias = _kind(bias_is_bf16, bias)
@@ -135,7 +135,7 @@ def _gemm_fused(fmt, M, N, K, A, SFA, B, SFB, D, alpha, bias, activation, gated,
     rc = getattr(load(), name)(
         M, N, K, _operand("A", A, M * K if fmt == "mxf8f4" else M * K // 2, dev),
         _operand("SFA", SFA, _blocked_bytes(M, K, vec), dev), _operand("B", B, N * K // 2, dev),
-        _operand("SFB", SFB, _blocked_bytes(N, K, vec), dev), _at("D", D, n, bf16, dev), alpha, epi,
+        _operand("SFB", SFB, _blocked_bytes(N, K, vec), dev), _at("D", D, n, bf16, dev), float(alpha), epi,
         SCHEDULES[schedule], _operand("workspace", workspace, 0, dev), workspace_bytes, handle)
     if rc != 0:
         raise BlackholeError(name, rc)
@@ -196,7 +196,7 @@ def gemm_fused_backward(M: int, N: int, dD, Z, dZ, dbias=None, activation: str =
     dD: BF16 of D's shape.  dZ may be Z, or dD when not gated.  workspace:
     gemm_fused_backward_workspace_bytes bytes, or None: allocated for this call from torch's
     caching allocator on the current stream."""
-    dev = _device()
+    M, N, dev = int(M), int(N), _device()
     handle, bf16 = _handle(stream, dev), _torch.bfloat16
     p_db = _at("dbias", dbias, N, _torch.float32, dev)
     need = gemm_fused_backward_workspace_bytes(M, N) if p_db and workspace is None else 0

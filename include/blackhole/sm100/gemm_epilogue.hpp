@@ -13,6 +13,11 @@
 //
 // Backward, from the stored Z:  dZ = dD * act'(Z), gated dZ[:, 2j] = dD act'(g) u and
 // dZ[:, 2j + 1] = dD act(g);  dbias = sum of its rows.  Bound by its bytes.
+//
+// Measured on B200: 8192^3 NVFP4 without any of it 209 us, SwiGLU 203, bias + GELU + residual 249
+// (plain product 203: the epilogue of a tile runs beside the next tile's products, and costs where
+// it is longer or competes for issue slots); M = 1, N = 28672, K = 8192 SwiGLU 24.5 us (plain
+// 23.4).  Backward, 8192 x 28672 SwiGLU: 1.17 GB in 190-197 us (0.91-0.95 of the measured copy rate).
 // =====================================================================================
 
 #include <cmath>

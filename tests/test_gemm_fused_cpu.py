@@ -88,3 +88,14 @@ def test_tensors_are_checked():
         forward(CALLS[0], D=torch.zeros(16, 128, dtype=torch.bfloat16))       # not on a GPU
     with pytest.raises(TypeError):
         forward(CALLS[0], bias=[0.0] * 256)
+
+
+def test_numpy_numbers_are_taken():
+    import numpy as np
+    for call in CALLS:
+        with pytest.raises(bh.BlackholeError):                       # refused by the library, not by ctypes
+            forward(call, M=np.int64(0), N=np.int32(256), K=np.int64(256), alpha=np.float32(0.5), beta=np.float32(1))
+    with pytest.raises(bh.BlackholeError):
+        bh.gemm_fused_backward(np.int64(0), np.int64(256), A, A + S, A + 2 * S, stream=0)
+    with pytest.raises(bh.BlackholeError):
+        bh.block_norm(np.int64(0), np.int64(256), A, A + S, eps=np.float32(1e-6), stream=0)
